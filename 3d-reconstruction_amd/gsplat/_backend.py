@@ -129,6 +129,16 @@ _SIGNATURES = {
     "gs_opacity_reset": (ctypes.c_int, [c_int64, c_float, _P, _P, _P, _P]),
     "gs_cube_texture_fwd": (ctypes.c_int, [c_int64, c_int32, c_int32, _P, _P, _P, _P, _P]),
     "gs_cube_texture_bwd": (ctypes.c_int, [c_int64, c_int32, c_int32, _P, _P, _P, _P, _P]),
+    "gs_embedding_fwd": (ctypes.c_int, [c_int64] * 3 + [c_int32, _P, c_int64, _P, c_int32, c_float, _P, _P]),
+    "gs_embedding_bwd_workspace_bytes": (c_int64, [c_int64] * 3),
+    "gs_embedding_bwd": (ctypes.c_int, [c_int64] * 3 + [c_int32, _P, c_int32, _P, c_int64, c_float, _P, c_int64, _P, _P]),
+    "gs_label_log_probs_workspace_bytes": (c_int64, [c_int64, c_int32, c_int32]),
+    "gs_label_log_probs_fwd": (ctypes.c_int, [c_int64, c_int32, c_int32, c_int32, _P, c_int64, _P, c_int32, _P, c_int64] +
+                               [_P] * 6),
+    "gs_label_log_probs_bwd": (ctypes.c_int, [c_int64, c_int32, c_int32, c_int32, _P, c_int64, _P, c_int32] + [_P] * 8),
+    "gs_grad_norm_workspace_bytes": (c_int64, [c_int32]),
+    "gs_grad_norm": (ctypes.c_int, [c_int32, _P, _P, _P, _P, c_int64, _P, _P]),
+    "gs_grad_clip": (ctypes.c_int, [c_int32, _P, _P, _P, _P, c_float, c_float, _P, c_int64, _P, _P]),
     "gs_mark_visible": (ctypes.c_int, [c_int64, _P, _P, _P]),
     "gs_compact_visible": (ctypes.c_int, [c_int32, c_int32] + [_P] * 10 + [_P]),
 }
@@ -288,6 +298,24 @@ class timed:
             b.record(torch.cuda.current_stream(self.dev))
             _prof.setdefault(self.name, []).append((self.a, b))
         return False
+
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # GS_DTYPE_*
+
+
+def dtype_code(t: torch.Tensor) -> int:
+    """GS_DTYPE_* of a tensor whose type the entry points with a `dtype` take."""
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"gsplat (MI355X build): float32, bfloat16 or float16 expected, got {t.dtype}")
+    return code
+
+
+def index_bytes(t: torch.Tensor) -> int:
+    """Bytes of an index: ids and labels are int64 or int32."""
+    if t.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"gsplat (MI355X build): int64 or int32 expected, got {t.dtype}")
+    return t.element_size()
 
 
 def f32c(t: torch.Tensor) -> torch.Tensor:

@@ -55,6 +55,11 @@ extern "C" {
 #define GS_ERR_NOT_POSTED (-4) /* gs_host_post_wait: the stream finished without the kernels having posted */
 #define GS_ERR_CONTRACT (-5)   /* a kernel found device-side inputs violating a documented precondition (below) */
 
+/* element types of the entry points that take one (the others are fp32) */
+#define GS_DTYPE_F32 0
+#define GS_DTYPE_BF16 1
+#define GS_DTYPE_F16 2
+
 /* colour source of gs_projection_fwd/_bwd */
 #define GS_COLOR_NONE 0 /* no colour input (render_mode "D"/"ED")                    */
 #define GS_COLOR_N 1    /* colors [N, color_dim], shared by all cameras               */
@@ -679,6 +684,51 @@ int gs_cube_texture_fwd(int64_t n, int32_t R, int32_t C, const float* tex, const
 /* v_tex [6,R,R,C] (zeroed by the caller) += the transpose of the lookup applied to v_out [n,C]. */
 int gs_cube_texture_bwd(int64_t n, int32_t R, int32_t C, const float* dirs, const float* rot, const float* v_out,
                         float* v_tex, void* stream);
+
+/* ---- learned codes: embedding lookup with scaling, and its gradient --------------------------------------- */
+/* out[i] = scale * table[ids[i]] over n ids and V rows of D elements (the appearance code of an image, the code of the
+ * instance a Gaussian belongs to: R/models/modules.py's embeddings are such tables); an id outside [0, V) selects
+ * nothing and gives a row of zeros.  `table` has rows `table_stride` elements apart, `out` is dense [n,D]; `ids` are
+ * int32 (id_bytes 4) or int64 (8); dtype: GS_DTYPE_*. */
+int gs_embedding_fwd(int64_t n, int64_t V, int64_t D, int32_t dtype, const void* table, int64_t table_stride,
+                     const void* ids, int32_t id_bytes, float scale, void* out, void* stream);
+/* v_table [V,D] (dense, written whole) = scale * the sum of the v_out rows (v_out_stride elements apart) of each id.
+ * Sums in fp32, in an order the ids alone fix, rounded once.  n < 2^30, V < 2^31. */
+int64_t gs_embedding_bwd_workspace_bytes(int64_t n, int64_t V, int64_t D);
+int gs_embedding_bwd(int64_t n, int64_t V, int64_t D, int32_t dtype, const void* ids, int32_t id_bytes,
+                     const void* v_out, int64_t v_out_stride, float scale, void* workspace /* 16-B aligned */,
+                     int64_t workspace_bytes, void* v_table, void* stream);
+
+/* ---- class channels: log probabilities of labels, entropy, top alternatives ------------------------------------ */
+/* Per row of K logits (rows `row_stride` elements apart): log_prob = log softmax at the row's label, entropy of the
+ * softmax, stats = {max, log of the sum of exp(x - max)} (kept for the backward), and the top_k largest log probabilities with their classes
+ * (descending, equal logits by the lower class, NaN first).  A label outside [0, K) gives log_prob 0.  A row of nothing
+ * but -inf has log probabilities -inf and entropy 0.  Outputs fp32; top_labels int64; top_k <= min(K,
+ * GS_LABEL_TOP_MAX), 0: the two top_* may be NULL. */
+#define GS_LABEL_TOP_MAX 64
+int64_t gs_label_log_probs_workspace_bytes(int64_t rows, int32_t K, int32_t top_k);
+int gs_label_log_probs_fwd(int64_t rows, int32_t K, int32_t dtype, int32_t top_k, const void* logits, int64_t row_stride,
+                           const void* labels, int32_t label_bytes, void* workspace, int64_t workspace_bytes,
+                           float* log_prob /* [rows] */, float* entropy /* [rows] */, float* stats /* [rows,2] */,
+                           float* top_log_probs /* [rows,top_k] */, int64_t* top_labels /* [rows,top_k] */, void* stream);
+/* v_logits [rows,K] (dense, written whole) from the gradients of log_prob, entropy and top_log_probs, each of which may
+ * be NULL.  Labels outside [0, K) and rows of nothing but -inf pass nothing on. */
+int gs_label_log_probs_bwd(int64_t rows, int32_t K, int32_t dtype, int32_t top_k, const void* logits, int64_t row_stride,
+                           const void* labels, int32_t label_bytes, const float* lse, const float* entropy,
+                           const int64_t* top_labels, const float* g_log_prob, const float* g_entropy,
+                           const float* g_top_log_probs, void* v_logits, void* stream);
+
+/* ---- gradients of a step: global norm and clipping ------------------------------------------------------- */
+/* norm [1] = sqrt of the sum of squares over all tensors (64-bit sums, order fixed by the sizes).  The *_host arrays are
+ * HOST arrays of n_tensors device pointers, element counts and GS_DTYPE_* codes; they are read before the call returns. */
+int64_t gs_grad_norm_workspace_bytes(int32_t n_tensors);
+int gs_grad_norm(int32_t n_tensors, const void* const* src_host, const int64_t* numel_host, const int32_t* dtype_host,
+                 void* workspace, int64_t workspace_bytes, float* norm, void* stream);
+/* norm as above, then dst_t = src_t * min(1, max_norm / (norm + eps)); dst_t == src_t scales in place (and leaves the
+ * tensors unread and unwritten when all are in place and the factor is 1).  No dst may overlap another tensor. */
+int gs_grad_clip(int32_t n_tensors, const void* const* src_host, void* const* dst_host, const int64_t* numel_host,
+                 const int32_t* dtype_host, float max_norm, float eps, void* workspace, int64_t workspace_bytes,
+                 float* norm, void* stream);
 
 #ifdef __cplusplus
 }
