@@ -8,46 +8,60 @@
 // A label outside [0, K) has no term: log_prob 0 and no gradient through it.  Logits of -inf have p = 0 and add nothing;
 // a row of nothing but -inf has log probabilities -inf, entropy 0 and no gradient.  NaN, or +inf, makes its row NaN.
 // The top alternatives are the largest logits, NaN above all, equal ones by the lower index.
+#include <algorithm>
+#include <type_traits>
+
 #include "dtype_io.hpp"
 
 namespace gs {
 
 constexpr int LP_THREADS = 256;
+constexpr int LP_SMALL = 64;       // classes up to which a lane takes a whole row
+constexpr int LP_WAVE = 2048;      // classes up to which a wave holds a row in registers
+constexpr int LP_SEGMENTS = 64;    // parts a long row is cut into at most
+constexpr int LP_LIST = 1024;      // candidates for the top alternatives that a workgroup lists
 constexpr float LP_LOG2E = 1.44269504088896340736f;
+constexpr float LP_LOW = -1.0e4f;  // stands for -inf next to an exponential that is 0 there: 0 * LP_LOW is 0
 
 __device__ __forceinline__ float lp_exp(float d) { return __builtin_amdgcn_exp2f(d * LP_LOG2E); }
 
-// max, sum of exp(x - max) and sum of exp(x - max) (x - max) of a part of a row
+// max, sum of exp(x - max) and sum of exp(x - max) (x - max) of a part of a row.  m ignores NaN, which s and w keep; with
+// nothing but -inf (and NaN) m stays -inf.
 struct LpStat {
   float m, s, w;
 };
 
-// the statistics of two parts; scaling m down to a new maximum shifts w by (m_old - m_new) s
-__device__ __forceinline__ LpStat lp_join(const LpStat& a, const LpStat& b) {
-  const float m = fmaxf(a.m, b.m);
-  if (m == -INFINITY) return {m, a.s + b.s, a.w + b.w};  // nothing but -inf so far (or NaN, which s keeps)
-  LpStat r{m, 0.f, 0.f};
-  const float da = a.m - m, db = b.m - m;
-  const float ea = a.m == -INFINITY ? 0.f : lp_exp(da), eb = b.m == -INFINITY ? 0.f : lp_exp(db);
-  r.s = a.s * ea + b.s * eb;
-  r.w = (ea == 0.f ? 0.f : ea * (a.w + da * a.s)) + (eb == 0.f ? 0.f : eb * (b.w + db * b.s));
-  return r;
+// adds N values; the sums are taken relative to the new maximum, by which w shifts by (m_old - m_new) s
+template <int N> __device__ __forceinline__ void lp_add(LpStat& st, const float (&x)[N]) {
+  float m = st.m;
+#pragma unroll
+  for (int k = 0; k < N; ++k) m = fmaxf(m, x[k]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  const float d = st.m - ref, e = lp_exp(d);  // 0 while there is nothing
+  float w = e * (st.w + fmaxf(d, LP_LOW) * st.s), s = e * st.s;
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const float dk = x[k] - ref, ek = lp_exp(dk);
+    s += ek;
+    w += ek * fmaxf(dk, LP_LOW);
+  }
+  st = {m, s, w};
 }
 
-__device__ __forceinline__ void lp_add(LpStat& st, float x) {
-  if (x > st.m) {
-    const float d = st.m - x;
-    const float e = st.m == -INFINITY ? 0.f : lp_exp(d);
-    st.w = e == 0.f ? 0.f : e * (st.w + d * st.s);
-    st.s *= e;
-    st.m = x;
+__device__ __forceinline__ LpStat lp_join(const LpStat& a, const LpStat& b) {
+  const float m = fmaxf(a.m, b.m);
+  const float ref = m == -INFINITY ? 0.f : m;
+  const float da = a.m - ref, db = b.m - ref, ea = lp_exp(da), eb = lp_exp(db);
+  return {m, ea * a.s + eb * b.s, ea * (a.w + fmaxf(da, LP_LOW) * a.s) + eb * (b.w + fmaxf(db, LP_LOW) * b.s)};
+}
+
+__device__ __forceinline__ LpStat lp_wave_join(LpStat st) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const LpStat b{__shfl_xor(st.m, o), __shfl_xor(st.s, o), __shfl_xor(st.w, o)};
+    st = lp_join(st, b);
   }
-  if (x != -INFINITY) {
-    const float d = x - st.m;
-    const float e = lp_exp(d);
-    st.s += e;
-    if (e != 0.f) st.w += e * d;
-  }
+  return st;
 }
 
 // a total order of logits: larger first, NaN above all, equal values (and the two zeros) by the lower index
@@ -56,7 +70,11 @@ __device__ __forceinline__ uint32_t lp_order(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);  // -0 becomes +0
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float lp_value(uint32_t order) {  // of an order that is not NaN's
+  return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
+}
 __device__ __forceinline__ uint64_t lp_key(float x, uint32_t j) { return ((uint64_t)lp_order(x) << 32) | (uint32_t)~j; }
+__device__ __forceinline__ uint32_t lp_key_index(uint64_t key) { return ~(uint32_t)key; }
 
 __device__ __forceinline__ uint64_t lp_wave_max(uint64_t v) {
 #pragma unroll
@@ -67,9 +85,40 @@ __device__ __forceinline__ uint64_t lp_wave_max(uint64_t v) {
   return v;
 }
 
+// the k-th largest of the lanes' values, bit by bit
+__device__ __forceinline__ uint32_t lp_wave_kth(uint32_t v, int k) {
+  uint32_t found = 0;
+#pragma unroll
+  for (int b = 31; b >= 0; --b) {
+    const uint32_t want = (found >> b) | 1u;
+    const int c = __popcll(__ballot((v >> b) == want));
+    if (c >= k) found |= 1u << b; else k -= c;
+  }
+  return found;
+}
+
 __device__ __forceinline__ int64_t lp_label(const void* labels, int label_bytes, int64_t r) {
   return label_bytes == 8 ? ((const int64_t*)labels)[r] : (int64_t)((const int32_t*)labels)[r];
 }
+
+// n values from x on, as a head up to the first 16-byte boundary, whole vectors and a tail: every row of an odd number of
+// classes starts at another alignment.  The head and the tail (fewer than 16 values) are a lane's single extra value each.
+template <typename T> struct LpSpan {
+  static constexpr int VE = 16 / (int)sizeof(T);
+  const T* x;
+  int n, head, vecs;
+  __device__ LpSpan(const T* p, int count) : x(p), n(count) {
+    const int h = (int)(((16u - ((uintptr_t)p & 15u)) & 15u) / sizeof(T));
+    head = h < n ? h : n;
+    vecs = (n - head) / VE;
+  }
+  __device__ int at(int v) const { return head + v * VE; }  // index of vector v's first value
+  __device__ int extra(int t) const {                       // index of thread t's extra value, -1: none
+    const int i = t < head ? t : head + vecs * VE + (t - head);
+    return i < n ? i : -1;
+  }
+  __device__ void load(int v, float (&f)[VE]) const { load_vec<T, VE>(x + at(v), f); }
+};
 
 struct LpFwd {
   int64_t rows, stride;
@@ -82,49 +131,371 @@ struct LpFwd {
 // (x - m) - log S, and what it is in a row of nothing but -inf
 __device__ __forceinline__ float lp_log_p(float x, float m, float ls) { return ls == -INFINITY ? -INFINITY : (x - m) - ls; }
 
-template <typename T>
-__device__ __forceinline__ void lp_write_row(const LpFwd& a, int64_t r, const LpStat& st, float ls, const T* x) {
-  a.stats[2 * r] = st.m;
-  a.stats[2 * r + 1] = ls;
+// `ls` = log S: -inf for a row of nothing but -inf, as for no other
+__device__ __forceinline__ void lp_write_row(const LpFwd& a, int64_t r, const LpStat& st, float ls, int64_t y, float x_y) {
+  *reinterpret_cast<float2*>(a.stats + 2 * r) = make_float2(st.m, ls);
   a.entropy[r] = ls == -INFINITY ? 0.f : ls - st.w / st.s;
-  const int64_t y = lp_label(a.labels, a.label_bytes, r);
-  a.log_prob[r] = y < 0 || y >= a.K ? 0.f : lp_log_p((float)x[y], st.m, ls);
+  a.log_prob[r] = y < 0 || y >= a.K ? 0.f : lp_log_p(x_y, st.m, ls);
 }
 
-// one wave per row
 template <typename T>
+__device__ __forceinline__ void lp_write_row(const LpFwd& a, int64_t r, const LpStat& st, float ls, const T* x) {
+  const int64_t y = lp_label(a.labels, a.label_bytes, r);
+  lp_write_row(a, r, st, ls, y, y < 0 || y >= a.K ? 0.f : (float)x[y]);
+}
+
+__device__ __forceinline__ void lp_write_top(const LpFwd& a, int64_t r, int rank, uint32_t j, float x, float m, float ls) {
+  a.top_idx[r * a.top + rank] = (int64_t)j;
+  a.top_lp[r * a.top + rank] = lp_log_p(x, m, ls);
+}
+
+// ------------------------------------------------------------------------------------------- up to LP_SMALL classes
+// A wave takes 64 rows: it reads their logits as one stretch, lane after lane, into LDS (rows an odd number of words
+// apart: lanes that each walk their own row hit different banks), and each lane works on one row without any exchange.
+// f / K for f < 64 K by a multiplication: (2^22 / K + 1) f is off by less than f / 2^22 < 1 / K.
+template <typename T>
+__device__ __forceinline__ void lp_small_load(const T* __restrict__ logits, int64_t stride, int64_t row0, int rows, int K,
+                                              int P, uint32_t magic, int lane, float* __restrict__ tile) {
+  const T* base = logits + row0 * stride;
+  const int total = rows * K;
+#pragma unroll 8
+  for (int f = lane; f < total; f += 64) {
+    const int r = (int)(((uint32_t)f * magic) >> 22);
+    const int c = f - r * K;
+    tile[r * P + c] = (float)base[r * stride + c];
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+template <typename T>
+__global__ __launch_bounds__(64) void label_small_fwd_kernel(LpFwd a, uint32_t magic, const T* __restrict__ logits) {
+  extern __shared__ float tile[];
+  const int lane = threadIdx.x, K = a.K, P = K | 1;
+  for (int64_t row0 = (int64_t)blockIdx.x * 64; row0 < a.rows; row0 += (int64_t)gridDim.x * 64) {
+    const int rows = (int)(a.rows - row0 < 64 ? a.rows - row0 : 64);
+    lp_small_load(logits, a.stride, row0, rows, K, P, magic, lane, tile);
+    if (lane < rows) {
+      const float* x = tile + lane * P;
+      const int64_t r = row0 + lane;
+      LpStat st{-INFINITY, 0.f, 0.f};
+      for (int j = 0; j < K; ++j) st.m = fmaxf(st.m, x[j]);
+      const float ref = st.m == -INFINITY ? 0.f : st.m;
+      for (int j = 0; j < K; ++j) {
+        const float d = x[j] - ref, e = lp_exp(d);
+        st.s += e;
+        st.w += e * fmaxf(d, LP_LOW);
+      }
+      const float ls = logf(st.s);
+      const int64_t y = lp_label(a.labels, a.label_bytes, r);
+      lp_write_row(a, r, st, ls, y, y < 0 || y >= K ? 0.f : x[y]);
+      uint64_t below = ~0ull;
+      for (int t = 0; t < a.top; ++t) {
+        uint64_t best = 0;
+        for (int j = 0; j < K; ++j) {
+          const uint64_t k = lp_key(x[j], (uint32_t)j);
+          if (k < below && k > best) best = k;
+        }
+        below = best;
+        const uint32_t j = lp_key_index(best);
+        lp_write_top(a, r, t, j, x[j], st.m, ls);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// -------------------------------------------------------------------------------------------- up to LP_WAVE classes
+// A wave holds a row in registers: NV vectors a lane and one extra value.  Read once, whatever is asked for.
+template <typename T, int NV>
 __global__ __launch_bounds__(LP_THREADS) void label_wave_fwd_kernel(LpFwd a, const T* __restrict__ logits) {
+  using Span = LpSpan<T>;
+  constexpr int VE = Span::VE, NX = NV * VE + 1;
+  __shared__ uint64_t lists[LP_THREADS];
+  uint64_t* list = lists + (threadIdx.x & ~63u);
   const int lane = threadIdx.x & 63;
   const int64_t waves = (int64_t)gridDim.x * (LP_THREADS / 64);
   for (int64_t r = (int64_t)blockIdx.x * (LP_THREADS / 64) + (threadIdx.x >> 6); r < a.rows; r += waves) {
-    const T* x = logits + r * a.stride;
-    LpStat st{-INFINITY, 0.f, 0.f};
-    for (int64_t j = lane; j < a.K; j += 64) lp_add(st, (float)x[j]);
+    const Span sp(logits + r * a.stride, a.K);
+    float x[NX];
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const LpStat b{__shfl_xor(st.m, o), __shfl_xor(st.s, o), __shfl_xor(st.w, o)};
-      st = lp_join(st, b);
-    }
-    const float ls = logf(st.s);  // -inf for a row of nothing but -inf, as for no other
-    if (lane == 0) lp_write_row(a, r, st, ls, x);
-    uint64_t below = ~0ull;
-    for (int t = 0; t < a.top; ++t) {
-      uint64_t best = 0;
-      for (int64_t j = lane; j < a.K; j += 64) {
-        const uint64_t k = lp_key((float)x[j], (uint32_t)j);
-        if (k < below && k > best) best = k;
+    for (int i = 0; i < NX; ++i) x[i] = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+      if (u * 64 + lane < sp.vecs) sp.load(u * 64 + lane, *reinterpret_cast<float(*)[VE]>(&x[u * VE]));
+    const int ex = sp.extra(lane);
+    if (ex >= 0) x[NX - 1] = (float)sp.x[ex];
+    LpStat st{-INFINITY, 0.f, 0.f};
+    lp_add<NX>(st, x);
+    const float lane_max = st.m;
+    st = lp_wave_join(st);
+    const float ls = logf(st.s);
+    if (lane == 0) lp_write_row(a, r, st, ls, sp.x);
+    if (a.top == 0) continue;
+    // the index of a lane's value, -1 where it has none
+    auto index = [&](int i) {
+      if (i == NX - 1) return ex;
+      const int v = (i / VE) * 64 + lane;
+      return v < sp.vecs ? sp.at(v) + i % VE : -1;
+    };
+    // The k-th largest of the lanes' maxima is no larger than the k-th largest value: what is not below it is listed.
+    int listed = 65;
+    if (st.s == st.s) {  // (NaN is above all, and no lane's maximum shows it: such rows go the long way)
+      const float least = lp_value(lp_wave_kth(lp_order(lane_max), a.top));
+      listed = 0;
+#pragma unroll
+      for (int i = 0; i < NX; ++i) {
+        const int j = index(i);
+        const bool in = j >= 0 && x[i] >= least;
+        const unsigned long long b = __ballot(in);
+        if (b) {
+          const int at = listed + __popcll(b & ((1ull << lane) - 1ull));
+          if (in && at < 64) list[at] = lp_key(x[i], (uint32_t)j);
+          listed += __popcll(b);
+        }
       }
-      best = lp_wave_max(best);
-      below = best;
-      if (lane == 0) {
-        const int64_t j = (int64_t)(uint32_t)~(uint32_t)best;
-        a.top_idx[r * a.top + t] = j;
-        a.top_lp[r * a.top + t] = lp_log_p((float)x[j], st.m, ls);
+    }
+    if (listed <= 64) {  // each lane ranks one of them
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      const uint64_t mine = lane < listed ? list[lane] : 0ull;
+      int rank = 0;
+      for (int i = 0; i < listed; ++i) rank += list[i] > mine;
+      if (lane < listed && rank < a.top) {
+        const uint32_t j = lp_key_index(mine);
+        lp_write_top(a, r, rank, j, lp_value((uint32_t)(mine >> 32)), st.m, ls);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    } else {  // many equal values, or NaN: one alternative after another
+      uint64_t below = ~0ull;
+      for (int t = 0; t < a.top; ++t) {
+        uint64_t best = 0;
+#pragma unroll
+        for (int i = 0; i < NX; ++i) {
+          const int j = index(i);
+          const uint64_t k = j >= 0 ? lp_key(x[i], (uint32_t)j) : 0ull;
+          if (k < below && k > best) best = k;
+        }
+        best = lp_wave_max(best);
+        below = best;
+        const uint32_t j = lp_key_index(best);
+        if (lane == 0) lp_write_top(a, r, t, j, (float)sp.x[j], st.m, ls);
       }
     }
   }
 }
 
+// ------------------------------------------------------------------------------------------------------- long rows
+// A workgroup reads a segment of a row (all of it when there are rows enough to fill the card), four vectors a thread in
+// flight.  A thread's strip is every 256th vector; its maximum comes out of the statistics for nothing, and the k-th
+// largest of a wave's strip maxima is no larger than the k-th largest value: only strips that reach it are read again,
+// and what they hold from it on is listed and ranked.  Rows whose list overflows (very many equal values) or that hold
+// NaN take the alternatives one by one, each thread keeping its strip's best and reading the strip again when it won.
+struct LpPart {  // of one segment
+  float m, s, w, pad;
+};
+
+template <typename T> __device__ __forceinline__ LpStat lp_strip(const LpSpan<T>& sp) {
+  constexpr int VE = LpSpan<T>::VE;
+  LpStat st{-INFINITY, 0.f, 0.f};
+  int v = threadIdx.x;
+  for (; v + 3 * LP_THREADS < sp.vecs; v += 4 * LP_THREADS) {
+    float f[4 * VE];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) sp.load(v + u * LP_THREADS, *reinterpret_cast<float(*)[VE]>(&f[u * VE]));
+    lp_add<4 * VE>(st, f);
+  }
+  for (; v < sp.vecs; v += LP_THREADS) {
+    float f[VE];
+    sp.load(v, f);
+    lp_add<VE>(st, f);
+  }
+  const int ex = sp.extra(threadIdx.x);
+  if (ex >= 0) {
+    const float f[1] = {(float)sp.x[ex]};
+    lp_add<1>(st, f);
+  }
+  return st;
+}
+
+// f(value, index) over the thread's strip
+template <typename T, typename F> __device__ __forceinline__ void lp_walk(const LpSpan<T>& sp, F&& f) {
+  constexpr int VE = LpSpan<T>::VE;
+  for (int v = threadIdx.x; v < sp.vecs; v += LP_THREADS) {
+    float x[VE];
+    sp.load(v, x);
+#pragma unroll
+    for (int k = 0; k < VE; ++k) f(x[k], sp.at(v) + k);
+  }
+  const int ex = sp.extra(threadIdx.x);
+  if (ex >= 0) f((float)sp.x[ex], ex);
+}
+
+struct LpShared {
+  LpStat part[LP_THREADS / 64];
+  uint32_t least[LP_THREADS / 64];
+  uint64_t best[LP_THREADS / 64];
+  int listed;
+  uint64_t list[LP_LIST];
+};
+
+// out(rank, key) for the k largest of n distinct keys in LDS (zeros are no keys)
+template <typename F> __device__ __forceinline__ void lp_rank_list(const uint64_t* list, int n, int k, F&& out) {
+  for (int i = threadIdx.x; i < n; i += LP_THREADS) {
+    const uint64_t mine = list[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += list[j] > mine;
+    if (rank < k && mine) out(rank, mine);
+  }
+}
+
+// Largest of the workgroup's values, for all threads; two barriers.
+__device__ __forceinline__ uint64_t lp_block_max(uint64_t v, uint64_t* lds) {
+  v = lp_wave_max(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  uint64_t m = lds[0];
+#pragma unroll
+  for (int w = 1; w < LP_THREADS / 64; ++w) m = lds[w] > m ? lds[w] : m;
+  return m;
+}
+
+// out(rank, key) for the segment's largest `top` values, in any order of ranks; j0 = index of its first value
+template <typename T, typename F>
+__device__ __forceinline__ void lp_block_top(const LpSpan<T>& sp, uint32_t j0, int top, const LpStat& strip, bool nan,
+                                             LpShared& sh, F&& out) {
+  int listed = LP_LIST + 1;
+  if (!nan) {
+    const uint32_t kth = lp_wave_kth(lp_order(strip.m), top);
+    if ((threadIdx.x & 63) == 0) sh.least[threadIdx.x >> 6] = kth;
+    if (threadIdx.x == 0) sh.listed = 0;
+    __syncthreads();
+    uint32_t order = sh.least[0];
+#pragma unroll
+    for (int w = 1; w < LP_THREADS / 64; ++w) order = sh.least[w] > order ? sh.least[w] : order;
+    const float least = lp_value(order);
+    if (strip.m >= least)
+      lp_walk(sp, [&](float x, int j) {
+        if (x >= least) {
+          const int at = atomicAdd(&sh.listed, 1);
+          if (at < LP_LIST) sh.list[at] = lp_key(x, j0 + (uint32_t)j);
+        }
+      });
+    __syncthreads();
+    listed = sh.listed;
+  }
+  if (listed <= LP_LIST) {
+    lp_rank_list(sh.list, listed, top, out);
+    return;
+  }
+  uint64_t below = ~0ull, best = 0;
+  auto search = [&]() {
+    best = 0;
+    lp_walk(sp, [&](float x, int j) {
+      const uint64_t k = lp_key(x, j0 + (uint32_t)j);
+      if (k < below && k > best) best = k;
+    });
+  };
+  search();
+  for (int t = 0; t < top; ++t) {
+    const uint64_t won = lp_block_max(best, sh.best);
+    if (threadIdx.x == 0 && won) out(t, won);
+    if (won == best && won) {
+      below = won;
+      search();
+    }
+  }
+}
+
+template <typename T, bool TOP>
+__global__ __launch_bounds__(LP_THREADS) void label_long_fwd_kernel(LpFwd a, int segments, int seg_len,
+                                                                    const T* __restrict__ logits,
+                                                                    LpPart* __restrict__ parts, uint64_t* __restrict__ keys) {
+  __shared__ typename std::conditional<TOP, LpShared, LpStat[LP_THREADS / 64]>::type sh;
+  LpStat* stats;
+  if constexpr (TOP) stats = sh.part; else stats = sh;
+  const int64_t items = a.rows * segments;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t r = item / segments;
+    const int j0 = (int)(item % segments) * seg_len;
+    const T* row = logits + r * a.stride;
+    const LpSpan<T> sp(row + j0, a.K - j0 < seg_len ? a.K - j0 : seg_len);
+    const LpStat strip = lp_strip(sp);
+    LpStat st = lp_wave_join(strip);
+    if ((threadIdx.x & 63) == 0) stats[threadIdx.x >> 6] = st;
+    __syncthreads();
+    st = stats[0];
+#pragma unroll
+    for (int w = 1; w < LP_THREADS / 64; ++w) st = lp_join(st, stats[w]);
+    const float ls = logf(st.s);
+    if (threadIdx.x == 0) {
+      if (segments == 1) lp_write_row(a, r, st, ls, row);
+      else parts[item] = {st.m, st.s, st.w, 0.f};
+    }
+    if constexpr (TOP) {
+      if (segments > 1)
+        for (int t = sp.n + threadIdx.x; t < a.top; t += LP_THREADS) keys[item * a.top + t] = 0;  // it holds fewer
+      lp_block_top(sp, (uint32_t)j0, a.top, strip, st.s != st.s, sh, [&](int rank, uint64_t key) {
+        if (segments == 1) {
+          const uint32_t j = lp_key_index(key);
+          lp_write_top(a, r, rank, j, (float)row[j], st.m, ls);
+        } else {
+          keys[item * a.top + rank] = key;
+        }
+      });
+    }
+    __syncthreads();
+  }
+}
+
+// joins the segments of a row
+template <typename T, bool TOP>
+__global__ __launch_bounds__(LP_THREADS) void label_join_kernel(LpFwd a, int segments, const T* __restrict__ logits,
+                                                                const LpPart* __restrict__ parts,
+                                                                const uint64_t* __restrict__ keys) {
+  const int64_t r = blockIdx.x;
+  const T* row = logits + r * a.stride;
+  const int lane = threadIdx.x & 63;
+  static_assert(LP_SEGMENTS <= 64, "a lane takes one segment");
+  LpStat st{-INFINITY, 0.f, 0.f};
+  if (lane < segments) {
+    const LpPart p = parts[r * segments + lane];
+    st = {p.m, p.s, p.w};
+  }
+  st = lp_wave_join(st);
+  const float ls = logf(st.s);
+  if (threadIdx.x == 0) lp_write_row(a, r, st, ls, row);
+  if constexpr (TOP) {
+    __shared__ LpShared sh;
+    const int n = segments * a.top;
+    const uint64_t* mine = keys + r * n;
+    auto out = [&](int rank, uint64_t key) {
+      const uint32_t j = lp_key_index(key);
+      lp_write_top(a, r, rank, j, (float)row[j], st.m, ls);
+    };
+    if (n <= LP_LIST) {
+      for (int i = threadIdx.x; i < n; i += LP_THREADS) sh.list[i] = mine[i];
+      __syncthreads();
+      lp_rank_list(sh.list, n, a.top, out);
+    } else {
+      uint64_t below = ~0ull;
+      for (int t = 0; t < a.top; ++t) {
+        uint64_t best = 0;
+        for (int i = threadIdx.x; i < n; i += LP_THREADS) {
+          const uint64_t k = mine[i];
+          if (k < below && k > best) best = k;
+        }
+        below = lp_block_max(best, sh.best);
+        if (threadIdx.x == 0) out(t, below);
+      }
+    }
+  }
+}
+
+// -------------------------------------------------------------------------------------------------------- gradient
 struct LpBwd {
   int64_t rows, stride;
   int32_t K, top, label_bytes;
@@ -137,7 +508,8 @@ struct LpBwd {
 // what a row's gradient needs: v_x_j = p_j (c0 - c1 (log p_j + H)) + the terms at y and t_k
 struct LpRow {
   float m, ls, H, c0, c1, g;
-  int64_t y;
+  int64_t y;  // -1: no label
+  bool none;  // nothing but -inf
 };
 
 __device__ __forceinline__ LpRow lp_row(const LpBwd& a, int64_t r) {
@@ -145,8 +517,9 @@ __device__ __forceinline__ LpRow lp_row(const LpBwd& a, int64_t r) {
   w.m = a.stats[2 * r];
   w.ls = a.stats[2 * r + 1];
   w.H = a.entropy[r];
+  w.none = w.ls == -INFINITY;
   const int64_t y = lp_label(a.labels, a.label_bytes, r);
-  const bool kept = y >= 0 && y < a.K;
+  const bool kept = y >= 0 && y < a.K && !w.none;
   w.y = kept ? y : -1;
   w.g = kept && a.g_lp ? a.g_lp[r] : 0.f;
   w.c0 = -w.g;
@@ -158,8 +531,72 @@ __device__ __forceinline__ LpRow lp_row(const LpBwd& a, int64_t r) {
 
 __device__ __forceinline__ float lp_grad(const LpRow& w, float x) {
   const float d = (x - w.m) - w.ls;
-  const float p = lp_exp(d);
-  return p == 0.f ? 0.f : p * (w.c0 - w.c1 * (d + w.H));
+  return lp_exp(d) * (w.c0 - w.c1 * (fmaxf(d, LP_LOW) + w.H));  // NaN stays in the exponential
+}
+
+// v at the t-th alternative of row r, whole
+template <typename T> __device__ __forceinline__ T lp_grad_top(const LpBwd& a, const LpRow& w, int64_t r, int t, float x) {
+  const int64_t j = a.top_idx[r * a.top + t];
+  return (T)(lp_grad(w, x) + (j == w.y ? w.g : 0.f) + a.g_top[r * a.top + t]);
+}
+
+template <typename T>
+__global__ __launch_bounds__(64) void label_small_bwd_kernel(LpBwd a, uint32_t magic, const T* __restrict__ logits,
+                                                             T* __restrict__ v) {
+  extern __shared__ float tile[];
+  const int lane = threadIdx.x, K = a.K, P = K | 1;
+  for (int64_t row0 = (int64_t)blockIdx.x * 64; row0 < a.rows; row0 += (int64_t)gridDim.x * 64) {
+    const int rows = (int)(a.rows - row0 < 64 ? a.rows - row0 : 64);
+    lp_small_load(logits, a.stride, row0, rows, K, P, magic, lane, tile);
+    if (lane < rows) {
+      float* x = tile + lane * P;
+      const int64_t r = row0 + lane;
+      const LpRow w = lp_row(a, r);
+      for (int j = 0; j < K; ++j) x[j] = w.none ? 0.f : lp_grad(w, x[j]);
+      if (w.y >= 0) x[w.y] += w.g;
+      if (a.g_top && !w.none)
+        for (int t = 0; t < a.top; ++t) x[a.top_idx[r * a.top + t]] += a.g_top[r * a.top + t];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    T* out = v + row0 * K;
+    const int total = rows * K;
+#pragma unroll 8
+    for (int f = lane; f < total; f += 64) {
+      const int r = (int)(((uint32_t)f * magic) >> 22);
+      out[f] = (T)tile[r * P + f - r * K];
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// `lanes` threads (a wave, or a workgroup) over a part of a row; the gradient's row is as far apart from a 16-byte boundary
+// as the logits' (`wide`), or is written value by value
+template <typename T, int LANES>
+__device__ __forceinline__ void lp_grad_span(const LpSpan<T>& sp, const LpRow& w, int j0, int t, T* __restrict__ out) {
+  constexpr int VE = LpSpan<T>::VE;
+  const bool wide = (((uintptr_t)sp.x ^ (uintptr_t)out) & 15u) == 0;
+  const int y = (int)(w.y - j0);  // the label's place in this part, if it is in it
+  for (int v = t; v < sp.vecs; v += LANES) {
+    float f[VE];
+    sp.load(v, f);
+#pragma unroll
+    for (int k = 0; k < VE; ++k) f[k] = w.none ? 0.f : lp_grad(w, f[k]);
+    const int j = sp.at(v);
+    if (w.y >= 0 && (uint32_t)(y - j) < (uint32_t)VE) {
+#pragma unroll
+      for (int k = 0; k < VE; ++k) f[k] += y == j + k ? w.g : 0.f;
+    }
+    if (wide) {
+      store_vec<T, VE>(out + j, f);
+    } else {
+#pragma unroll
+      for (int k = 0; k < VE; ++k) out[j + k] = (T)f[k];
+    }
+  }
+  const int ex = sp.extra(t);
+  if (ex >= 0) out[ex] = (T)((w.none ? 0.f : lp_grad(w, (float)sp.x[ex])) + (w.y >= 0 && ex == y ? w.g : 0.f));
 }
 
 template <typename T>
@@ -167,19 +604,40 @@ __global__ __launch_bounds__(LP_THREADS) void label_wave_bwd_kernel(LpBwd a, con
   const int lane = threadIdx.x & 63;
   const int64_t waves = (int64_t)gridDim.x * (LP_THREADS / 64);
   for (int64_t r = (int64_t)blockIdx.x * (LP_THREADS / 64) + (threadIdx.x >> 6); r < a.rows; r += waves) {
-    const T* x = logits + r * a.stride;
-    T* o = v + r * a.K;
+    const LpSpan<T> sp(logits + r * a.stride, a.K);
     const LpRow w = lp_row(a, r);
-    const bool none = w.ls == -INFINITY;
-    for (int64_t j = lane; j < a.K; j += 64) {
-      float g = none ? 0.f : lp_grad(w, (float)x[j]);
-      if (!none) {
-        if (j == w.y) g += w.g;
-        if (a.g_top)
-          for (int t = 0; t < a.top; ++t)
-            if (a.top_idx[r * a.top + t] == j) g += a.g_top[r * a.top + t];
+    T* out = v + r * a.K;
+    lp_grad_span<T, 64>(sp, w, 0, lane, out);
+    if (a.g_top && !w.none) {
+      __builtin_amdgcn_s_waitcnt(0);  // the row's stores are out before some of its values are stored again
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+      if (lane < a.top) {
+        const int64_t j = a.top_idx[r * a.top + lane];
+        out[j] = lp_grad_top<T>(a, w, r, lane, (float)sp.x[j]);
       }
-      o[j] = (T)g;
+    }
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(LP_THREADS) void label_long_bwd_kernel(LpBwd a, int segments, int seg_len,
+                                                                    const T* __restrict__ logits, T* __restrict__ v) {
+  const int64_t items = a.rows * segments;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t r = item / segments;
+    const int j0 = (int)(item % segments) * seg_len;
+    const LpSpan<T> sp(logits + r * a.stride + j0, a.K - j0 < seg_len ? a.K - j0 : seg_len);
+    const LpRow w = lp_row(a, r);
+    T* out = v + r * a.K + j0;
+    lp_grad_span<T, LP_THREADS>(sp, w, j0, threadIdx.x, out);
+    if (a.g_top && !w.none) {
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+      if ((int)threadIdx.x < a.top) {
+        const int64_t j = a.top_idx[r * a.top + threadIdx.x] - j0;
+        if (j >= 0 && j < sp.n) out[j] = lp_grad_top<T>(a, w, r, threadIdx.x, (float)sp.x[j]);
+      }
+      __syncthreads();
     }
   }
 }
@@ -187,7 +645,7 @@ __global__ __launch_bounds__(LP_THREADS) void label_wave_bwd_kernel(LpBwd a, con
 static int lp_check(int64_t rows, int32_t K, int32_t dtype, int32_t top_k, const void* logits, int64_t row_stride,
                     const void* labels, int32_t label_bytes) {
   if (rows < 0 || K < 1 || !dtype_size(dtype) || top_k < 0 || top_k > K || row_stride < 0) return GS_ERR_INVALID_ARG;
-  if (top_k > GS_LABEL_TOP_MAX) return GS_ERR_UNSUPPORTED;
+  if (top_k > GS_LABEL_TOP_MAX || K > GS_LABEL_CLASSES_MAX) return GS_ERR_UNSUPPORTED;
   if (label_bytes != 4 && label_bytes != 8) return GS_ERR_INVALID_ARG;
   if (rows == 0) return GS_OK;
   if (!logits || !labels) return GS_ERR_INVALID_ARG;
@@ -196,14 +654,38 @@ static int lp_check(int64_t rows, int32_t K, int32_t dtype, int32_t top_k, const
   return GS_OK;
 }
 
-static unsigned lp_wave_grid(int64_t rows) {
-  const int64_t b = ceil_div(rows, LP_THREADS / 64);
-  return (unsigned)(b < (1 << 20) ? b : (1 << 20));
+static unsigned lp_grid(int64_t items, int per_block) {
+  const int64_t b = ceil_div(items, per_block);
+  return (unsigned)(b < (1 << 20) ? b : (1 << 20));  // (the kernels go on to further items)
 }
+
+// Segments of a long row: about a thousand workgroups in all (four a CU), none shorter than a vector for each thread.
+static int lp_segments(int64_t rows, int32_t K, int32_t* seg_len) {
+  int64_t n = rows >= 1024 ? 1 : ceil_div(1024, rows);
+  n = std::min<int64_t>(n, std::min<int64_t>(LP_SEGMENTS, ceil_div(K, 2048)));
+  *seg_len = (int32_t)(ceil_div(ceil_div(K, n), 64) * 64);
+  return (int)ceil_div(K, *seg_len);
+}
+
+template <typename F> static int with_vectors(int n, F&& f) {
+  if (n <= 1) return f(std::integral_constant<int, 1>{});
+  if (n <= 2) return f(std::integral_constant<int, 2>{});
+  if (n <= 4) return f(std::integral_constant<int, 4>{});
+  return f(std::integral_constant<int, 8>{});
+}
+
+static uint32_t lp_magic(int32_t K) { return (1u << 22) / (uint32_t)K + 1u; }
+
+static int64_t lp_parts_bytes(int64_t items) { return ceil_div(items * (int64_t)sizeof(LpPart), 256) * 256; }
 
 }  // namespace gs
 
-extern "C" int64_t gs_label_log_probs_workspace_bytes(int64_t rows, int32_t K, int32_t top_k) { return 0; }
+extern "C" int64_t gs_label_log_probs_workspace_bytes(int64_t rows, int32_t K, int32_t top_k) {
+  if (rows <= 0 || K <= gs::LP_WAVE || top_k < 0) return 0;
+  int32_t seg_len;
+  const int64_t segments = gs::lp_segments(rows, K, &seg_len);
+  return segments == 1 ? 0 : gs::lp_parts_bytes(rows * segments) + 8 * rows * segments * top_k;
+}
 
 extern "C" int gs_label_log_probs_fwd(int64_t rows, int32_t K, int32_t dtype, int32_t top_k, const void* logits,
                                       int64_t row_stride, const void* labels, int32_t label_bytes, void* workspace,
@@ -213,12 +695,46 @@ extern "C" int gs_label_log_probs_fwd(int64_t rows, int32_t K, int32_t dtype, in
   const int st = lp_check(rows, K, dtype, top_k, logits, row_stride, labels, label_bytes);
   if (st != GS_OK || rows == 0) return st;
   if (!log_prob || !entropy || !stats || (top_k > 0 && (!top_log_probs || !top_labels))) return GS_ERR_INVALID_ARG;
-  if (workspace_bytes < gs_label_log_probs_workspace_bytes(rows, K, top_k)) return GS_ERR_WORKSPACE;
+  if ((uintptr_t)stats & 7) return GS_ERR_INVALID_ARG;
+  const int64_t need = gs_label_log_probs_workspace_bytes(rows, K, top_k);
+  if (workspace_bytes < need) return GS_ERR_WORKSPACE;
+  if (need > 0 && (!workspace || ((uintptr_t)workspace & 15))) return GS_ERR_INVALID_ARG;
   const LpFwd a{rows, row_stride, K, top_k, label_bytes, labels, log_prob, entropy, stats, top_log_probs, top_labels};
+  hipStream_t s = (hipStream_t)stream;
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    hipLaunchKernelGGL(label_wave_fwd_kernel<T>, dim3(lp_wave_grid(rows)), dim3(LP_THREADS), 0, (hipStream_t)stream, a,
-                       (const T*)logits);
+    const T* x = (const T*)logits;
+    if (K <= LP_SMALL) {
+      hipLaunchKernelGGL(label_small_fwd_kernel<T>, dim3(lp_grid(rows, 64)), dim3(64), 64 * (K | 1) * sizeof(float), s, a,
+                         lp_magic(K), x);
+      GS_CHECK_LAUNCH();
+      return GS_OK;
+    }
+    if (K <= LP_WAVE)
+      return with_vectors((int)ceil_div(K, 64 * LpSpan<T>::VE), [&](auto nv) {
+        constexpr int NV = decltype(nv)::value;
+        if constexpr (NV * LpSpan<T>::VE * 64 <= LP_WAVE) {
+          hipLaunchKernelGGL((label_wave_fwd_kernel<T, NV>), dim3(lp_grid(rows, LP_THREADS / 64)), dim3(LP_THREADS), 0, s, a, x);
+          GS_CHECK_LAUNCH();
+          return GS_OK;
+        }
+        return GS_ERR_INVALID_ARG;
+      });
+    int32_t seg_len;
+    const int segments = lp_segments(rows, K, &seg_len);
+    LpPart* parts = (LpPart*)workspace;
+    uint64_t* keys = (uint64_t*)((char*)workspace + lp_parts_bytes(rows * segments));
+    const dim3 grid(lp_grid(rows * segments, 1)), block(LP_THREADS);
+    if (top_k > 0)
+      hipLaunchKernelGGL((label_long_fwd_kernel<T, true>), grid, block, 0, s, a, segments, seg_len, x, parts, keys);
+    else
+      hipLaunchKernelGGL((label_long_fwd_kernel<T, false>), grid, block, 0, s, a, segments, seg_len, x, parts, keys);
+    GS_CHECK_LAUNCH();
+    if (segments == 1) return GS_OK;
+    if (top_k > 0)
+      hipLaunchKernelGGL((label_join_kernel<T, true>), dim3((unsigned)rows), block, 0, s, a, segments, x, parts, keys);
+    else
+      hipLaunchKernelGGL((label_join_kernel<T, false>), dim3((unsigned)rows), dim3(64), 0, s, a, segments, x, parts, keys);
     GS_CHECK_LAUNCH();
     return GS_OK;
   });
@@ -234,10 +750,22 @@ extern "C" int gs_label_log_probs_bwd(int64_t rows, int32_t K, int32_t dtype, in
   if (!stats || !entropy || !v_logits || (g_top_log_probs && (top_k < 1 || !top_labels))) return GS_ERR_INVALID_ARG;
   if ((uintptr_t)v_logits & (uintptr_t)(dtype_size(dtype) - 1)) return GS_ERR_INVALID_ARG;
   const LpBwd a{rows, row_stride, K, top_k, label_bytes, labels, stats, entropy, top_labels, g_log_prob, g_entropy, g_top_log_probs};
+  hipStream_t s = (hipStream_t)stream;
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    hipLaunchKernelGGL(label_wave_bwd_kernel<T>, dim3(lp_wave_grid(rows)), dim3(LP_THREADS), 0, (hipStream_t)stream, a,
-                       (const T*)logits, (T*)v_logits);
+    const T* x = (const T*)logits;
+    if (K <= LP_SMALL) {
+      hipLaunchKernelGGL(label_small_bwd_kernel<T>, dim3(lp_grid(rows, 64)), dim3(64), 64 * (K | 1) * sizeof(float), s, a,
+                         lp_magic(K), x, (T*)v_logits);
+    } else if (K <= LP_WAVE) {
+      hipLaunchKernelGGL(label_wave_bwd_kernel<T>, dim3(lp_grid(rows, LP_THREADS / 64)), dim3(LP_THREADS), 0, s, a, x,
+                         (T*)v_logits);
+    } else {
+      int32_t seg_len;
+      const int segments = lp_segments(rows, K, &seg_len);
+      hipLaunchKernelGGL(label_long_bwd_kernel<T>, dim3(lp_grid(rows * segments, 1)), dim3(LP_THREADS), 0, s, a, segments,
+                         seg_len, x, (T*)v_logits);
+    }
     GS_CHECK_LAUNCH();
     return GS_OK;
   });

@@ -704,8 +704,9 @@ int gs_embedding_bwd(int64_t n, int64_t V, int64_t D, int32_t dtype, const void*
  * softmax, stats = {max, log of the sum of exp(x - max)} (kept for the backward), and the top_k largest log probabilities with their classes
  * (descending, equal logits by the lower class, NaN first).  A label outside [0, K) gives log_prob 0.  A row of nothing
  * but -inf has log probabilities -inf and entropy 0.  Outputs fp32; top_labels int64; top_k <= min(K,
- * GS_LABEL_TOP_MAX), 0: the two top_* may be NULL. */
+ * GS_LABEL_TOP_MAX), 0: the two top_* may be NULL.  K <= GS_LABEL_CLASSES_MAX. */
 #define GS_LABEL_TOP_MAX 64
+#define GS_LABEL_CLASSES_MAX (1 << 30)
 int64_t gs_label_log_probs_workspace_bytes(int64_t rows, int32_t K, int32_t top_k);
 int gs_label_log_probs_fwd(int64_t rows, int32_t K, int32_t dtype, int32_t top_k, const void* logits, int64_t row_stride,
                            const void* labels, int32_t label_bytes, void* workspace, int64_t workspace_bytes,
