@@ -300,22 +300,27 @@ class timed:
         return False
 
 
-_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # GS_DTYPE_*
+_ops = None
 
 
-def dtype_code(t: torch.Tensor) -> int:
-    """GS_DTYPE_* of a tensor whose type the entry points with a `dtype` take."""
-    code = _DTYPES.get(t.dtype)
-    if code is None:
-        raise TypeError(f"gsplat (MI355X build): float32, bfloat16 or float16 expected, got {t.dtype}")
-    return code
+def ops():
+    """Load (once) and return `_torch_ops` (csrc/torch_ops.cpp): arguments, workspaces and autograd nodes of the operators
+    whose calls are short, in C++ over the same native library."""
+    global _ops
+    if _ops is None:
+        from importlib.util import module_from_spec, spec_from_file_location
 
-
-def index_bytes(t: torch.Tensor) -> int:
-    """Bytes of an index: ids and labels are int64 or int32."""
-    if t.dtype not in (torch.int64, torch.int32):
-        raise TypeError(f"gsplat (MI355X build): int64 or int32 expected, got {t.dtype}")
-    return t.element_size()
+        path = os.path.normpath(os.path.join(os.path.dirname(_LIB_PATH), "_torch_ops.so"))
+        if not os.path.exists(path):
+            raise RuntimeError(f"_torch_ops.so not found at {path}: build it with `python -c 'import __graft_entry__ as g; "
+                               "g.build()'` (make -C 3d-reconstruction_amd/csrc).  There is no Python fallback.")
+        lib()
+        spec = spec_from_file_location("_torch_ops", path)
+        module = module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.load(lib_path())
+        _ops = module
+    return _ops
 
 
 def f32c(t: torch.Tensor) -> torch.Tensor:

@@ -14,7 +14,6 @@ from typing import NamedTuple, Optional, Tuple
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from . import _backend as B
 
@@ -305,51 +304,6 @@ class LabelLogProbs(NamedTuple):
     top_labels: Optional[Tensor]      # [..., top_k] their classes, int64
 
 
-class _LabelLogProbs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, labels, top_k):  # [rows,K], [rows]
-        dev = logits.device
-        rows, K = logits.shape
-        x = logits if K == 1 or logits.stride(1) == 1 else logits.contiguous()
-        y = labels.contiguous()
-        L = B.lib()
-        log_prob, entropy = (torch.empty(rows, device=dev, dtype=torch.float32) for _ in range(2))
-        stats = torch.empty(rows, 2, device=dev, dtype=torch.float32)
-        top_lp = torch.empty(rows, top_k, device=dev, dtype=torch.float32)
-        top_idx = torch.empty(rows, top_k, device=dev, dtype=torch.int64)
-        nbytes = int(L.gs_label_log_probs_workspace_bytes(rows, K, top_k))
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-        with B.device_guard(dev), B.timed("gs_label_log_probs_fwd", dev):
-            B.check(L.gs_label_log_probs_fwd(rows, K, B.dtype_code(x), top_k, B.ptr(x), x.stride(0), B.ptr(y),
-                                             B.index_bytes(y), B.ptr(ws), nbytes, B.ptr(log_prob), B.ptr(entropy),
-                                             B.ptr(stats), B.ptr(top_lp), B.ptr(top_idx), B.stream_handle(dev)),
-                    "gs_label_log_probs_fwd")
-        ctx.save_for_backward(x, y, stats, entropy, top_idx)
-        ctx.top_k = top_k
-        ctx.mark_non_differentiable(top_idx)
-        ctx.set_materialize_grads(False)
-        return log_prob, entropy, top_lp, top_idx
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g_lp, g_ent, g_top, _g_idx):
-        x, y, stats, entropy, top_idx = ctx.saved_tensors
-        if ctx.top_k == 0:
-            g_top = None
-        if g_lp is None and g_ent is None and g_top is None:
-            return None, None, None
-        dev = x.device
-        rows, K = x.shape
-        g_lp, g_ent, g_top = (None if g is None else B.f32c(g) for g in (g_lp, g_ent, g_top))
-        v = torch.empty(rows, K, device=dev, dtype=x.dtype)
-        with B.device_guard(dev), B.timed("gs_label_log_probs_bwd", dev):
-            B.check(B.lib().gs_label_log_probs_bwd(rows, K, B.dtype_code(x), ctx.top_k, B.ptr(x), x.stride(0), B.ptr(y),
-                                                   B.index_bytes(y), B.ptr(stats), B.ptr(entropy), B.ptr(top_idx),
-                                                   B.ptr(g_lp), B.ptr(g_ent), B.ptr(g_top), B.ptr(v),
-                                                   B.stream_handle(dev)), "gs_label_log_probs_bwd")
-        return v, None, None
-
-
 def label_log_probs(logits: Tensor, labels: Tensor, top_k: int = 0) -> LabelLogProbs:
     """Log probabilities of the given labels under `softmax(logits)`, with the entropy of each row and its `top_k` best
     alternatives, in one pass over the logits: per-pixel classes rendered as channels (`logits = render[..., 3:]`,
@@ -365,15 +319,8 @@ def label_log_probs(logits: Tensor, labels: Tensor, top_k: int = 0) -> LabelLogP
     top_log_probs."""
     assert logits.dim() >= 1 and logits.shape[-1] >= 1, f"logits must be [..., K], got {tuple(logits.shape)}"
     assert labels.shape == logits.shape[:-1], f"labels must be {tuple(logits.shape[:-1])}, got {tuple(labels.shape)}"
-    B.dtype_code(logits), B.index_bytes(labels)
     top_k = int(top_k)
     if not 0 <= top_k <= min(logits.shape[-1], 64):
         raise ValueError(f"top_k must be within 0..min(K, 64), got {top_k} for K = {logits.shape[-1]}")
-    B.require_gpu(logits, labels)
-    shape = labels.shape
-    if len(shape) != 1:
-        logits, labels = logits.reshape(labels.numel(), logits.shape[-1]), labels.reshape(-1)
-    res = _LabelLogProbs.apply(logits, labels, top_k)
-    if len(shape) != 1:
-        res = [t.reshape(shape + t.shape[1:]) for t in res]
-    return LabelLogProbs(res[0], res[1], res[2] if top_k else None, res[3] if top_k else None)
+    log_prob, entropy, top, top_labels = B.ops().label_log_probs(logits, labels, top_k)
+    return LabelLogProbs(log_prob, entropy, top if top_k else None, top_labels if top_k else None)

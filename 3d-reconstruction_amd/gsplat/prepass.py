@@ -20,7 +20,6 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from . import _backend as B
 
@@ -243,53 +242,13 @@ def rigid_transform(means: Tensor, quats: Tensor, point_ids: Tensor, inst_quats:
 # ---------------------------------------------------------------------------------------------------------------------
 # learned codes: embedding lookup
 
-class _EmbeddingLookup(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, table, ids, scale):
-        dev = B.require_gpu(table, ids)
-        V, D = table.shape
-        n = ids.numel()
-        flat = ids.reshape(n).contiguous()
-        rows = table if D == 0 or table.stride(1) == 1 else table.contiguous()
-        out = torch.empty(tuple(ids.shape) + (D,), device=dev, dtype=table.dtype)
-        with B.device_guard(dev), B.timed("gs_embedding_fwd", dev):
-            B.check(B.lib().gs_embedding_fwd(n, V, D, B.dtype_code(table), B.ptr(rows), rows.stride(0), B.ptr(flat),
-                                             B.index_bytes(flat), scale, B.ptr(out), B.stream_handle(dev)),
-                    "gs_embedding_fwd")
-        ctx.save_for_backward(flat)
-        ctx.geom = (n, V, D, scale, table.dtype)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, v_out):
-        (flat,) = ctx.saved_tensors
-        n, V, D, scale, dtype = ctx.geom
-        dev = flat.device
-        v = v_out.reshape(n, D) if n > 0 else v_out.new_empty(0, D)
-        if D > 1 and v.stride(1) != 1:
-            v = v.contiguous()
-        L = B.lib()
-        v_table = torch.empty(V, D, device=dev, dtype=dtype)
-        nbytes = int(L.gs_embedding_bwd_workspace_bytes(n, V, D))
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-        with B.device_guard(dev), B.timed("gs_embedding_bwd", dev):
-            B.check(L.gs_embedding_bwd(n, V, D, B.dtype_code(v_table), B.ptr(flat), B.index_bytes(flat), B.ptr(v),
-                                       v.stride(0), scale, B.ptr(ws), nbytes, B.ptr(v_table), B.stream_handle(dev)),
-                    "gs_embedding_bwd")
-        return v_table, None, None
-
-
 def embedding_lookup(table: Tensor, ids: Tensor, scale: float = 1.0, validate: bool = False) -> Tensor:
     """`scale * table[ids]`: the learned code of each image, or of the instance each Gaussian belongs to (`point_ids`).
     table [V,D] fp32, bf16 or fp16; ids of any shape, int64 or int32; returns [*ids.shape, D] in the table's type.  An id
     outside [0, V) (a Gaussian without an instance) gives a row of zeros and passes no gradient on; `validate=True` raises
-    for one instead (one host synchronisation).  Differentiable w.r.t. the table: the gradient is dense, each row the sum
-    over its ids in ascending position, in fp32, the same bits in every run."""
+    for one instead (one host synchronisation).  Differentiable once w.r.t. the table: the gradient is dense, each row the
+    sum over its ids in fp32, in an order that the ids alone fix: the same bits in every run."""
     assert table.dim() == 2, f"table must be [V,D], got {tuple(table.shape)}"
-    B.dtype_code(table), B.index_bytes(ids)
-    scale = float(scale)
-    B.require_gpu(table, ids)
     if validate and ids.numel() > 0 and not bool(((ids >= 0) & (ids < table.shape[0])).all()):
         raise IndexError(f"ids outside [0, {table.shape[0]})")
-    return _EmbeddingLookup.apply(table, ids, scale)
+    return B.ops().embedding_lookup(table, ids, scale)

@@ -218,5 +218,5 @@ def test_refusals_on_the_device(gpu_device):
         embedding_lookup(t, ids.cpu())
     leaf = t.clone().requires_grad_(True)
     (v,) = torch.autograd.grad(embedding_lookup(leaf, ids).square().sum(), leaf, create_graph=True)
-    with pytest.raises(RuntimeError, match="once_differentiable|differentiated twice|does not require grad"):
+    with pytest.raises(RuntimeError, match="cannot be differentiated twice"):
         v.sum().backward()

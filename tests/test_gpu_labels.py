@@ -339,7 +339,7 @@ def test_refusals_on_the_device(gpu_device):
         label_log_probs(x, y.cpu())
     leaf = x.clone().requires_grad_(True)
     (v,) = torch.autograd.grad(label_log_probs(leaf, y).log_prob.sum(), leaf, create_graph=True)
-    with pytest.raises(RuntimeError, match="once_differentiable|differentiated twice|does not require grad"):
+    with pytest.raises(RuntimeError, match="cannot be differentiated twice"):
         v.sum().backward()
     got = label_log_probs(leaf, y)
     with torch.no_grad():
