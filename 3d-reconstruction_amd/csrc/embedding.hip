@@ -2,22 +2,34 @@
 //   out[i] = scale * table[ids[i]]                          (an id outside [0, V) selects nothing: a row of zeros)
 //   v_table[v] = scale * sum over i with ids[i] = v, in ascending i, of v_out[i]
 // Both are bound by HBM.  The lookup reads n rows and writes n rows in the widest vectors that the row size and the
-// alignment allow.  The gradient reads every row of v_out once and writes every row of the table once:
-//   ids -> (id, position) pairs, stably sorted by id (gs_radix_sort_pairs_u64_u32_bits);
-//   embed_rows_kernel   owns rows of the table: finds each row's run in the sorted ids, adds its rows of v_out (or
-//                       writes zeros), leaves out the runs longer than EMB_LONG;
-//   embed_pieces_kernel cuts the sorted ids into pieces of EMB_LONG and adds up what of a long run lies in each;
-//   embed_join_kernel   adds the pieces of each long run.
+// alignment allow.  The gradient reads every row of v_out once and writes the table:
+//   1. the ids are sorted, stably, with their positions: by one workgroup in LDS up to EMB_SORT1 of them, else by a radix
+//      sort of three launches a digit.  The sort leaves most of the card idle, so its launches carry the zeros of the
+//      table along: workgroups behind those of the sort fill a share of it each.
+//   2. embed_runs_kernel cuts the sorted ids into pieces, one to a group of lanes as wide as a row.  A run of equal ids no
+//      longer than a piece is added up by the group in whose piece it starts, and stored; of a longer run each group adds
+//      what lies in its piece.
+//   3. embed_join_kernel adds the pieces of each long run.
 // Sums are held in fp32, taken in an order that the ids alone fix (no float atomics), and rounded once at the end.
 // Up to EMB_DIRECT ids need no sort: each workgroup picks the ids that fall among its rows of the table.
+#include <algorithm>
+#include <type_traits>
+
 #include "dtype_io.hpp"
 
 namespace gs {
 
 constexpr int EMB_THREADS = 256;
-constexpr int EMB_LONG = 64;
 constexpr int EMB_DIRECT = 256;
-constexpr int EMB_ROWS_MAX = 256;  // rows of the table per workgroup
+constexpr int EMB_ROWS_MAX = 256;     // rows of the table per workgroup of the direct form
+constexpr int EMB_SORT1 = 16384;      // ids that one workgroup sorts in LDS
+constexpr int EMB_SORT1_THREADS = 1024;
+constexpr int EMB_RADIX_BITS = 9;
+constexpr int EMB_RADIX = 1 << EMB_RADIX_BITS;
+constexpr int EMB_ITEMS = 8;          // ids per thread and launch of the radix sort
+constexpr int EMB_TILE = EMB_THREADS * EMB_ITEMS;
+constexpr int EMB_JOIN_THREADS = 1024;
+constexpr int EMB_JOIN_PIECES = 16;   // pieces that a workgroup of the join looks at
 
 __device__ __forceinline__ int64_t emb_id(const void* ids, int id_bytes, int64_t i) {
   return id_bytes == 8 ? ((const int64_t*)ids)[i] : (int64_t)((const int32_t*)ids)[i];
@@ -25,7 +37,7 @@ __device__ __forceinline__ int64_t emb_id(const void* ids, int id_bytes, int64_t
 
 // ---------------------------------------------------------------------------------------------------------- lookup
 // vpr vectors of N elements per row; a workgroup takes `rows_per` rows at a time, their vectors numbered through.
-// f / vpr by a multiplication: exact while f * vpr < 2^32 (the host keeps rows_per * vpr at 4096, or rows_per at 1).
+// f / vpr by a multiplication: exact while f * vpr < 2^32 (f is below 2048, vpr too unless rows_per is 1).
 template <typename T, int N>
 __global__ __launch_bounds__(EMB_THREADS) void embed_lookup_kernel(int64_t n, int64_t V, int64_t vpr, int rows_per,
                                                                    uint32_t magic, const T* __restrict__ table,
@@ -63,7 +75,7 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_lookup_kernel(int64_t n, in
 struct EmbShape {
   int64_t n, V, vpr;  // ids, rows of the table, vectors per row
   int64_t gs;         // row stride of v_out in elements
-  int32_t G, rows_per;
+  int32_t G, rows_per, piece;
   float scale;
 };
 
@@ -75,23 +87,6 @@ __device__ __forceinline__ void emb_add(float (&acc)[N], const T* __restrict__ v
   for (int k = 0; k < N; ++k) acc[k] += x[k];
 }
 
-// sum of v_out over the sorted entries [s, e), in order, four rows in flight
-template <typename T, int N>
-__device__ __forceinline__ void emb_sum(float (&acc)[N], const uint32_t* __restrict__ pos, int64_t s, int64_t e,
-                                        const T* __restrict__ v_out, int64_t gs, int64_t col) {
-  int64_t i = s;
-  for (; i + 4 <= e; i += 4) {
-    float x[4][N];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) load_vec<T, N>(v_out + (int64_t)pos[i + u] * gs + col, x[u]);
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int k = 0; k < N; ++k) acc[k] += x[u][k];
-  }
-  for (; i < e; ++i) emb_add<T, N>(acc, v_out, gs, (int64_t)pos[i], col);
-}
-
 template <typename T, int N>
 __device__ __forceinline__ void emb_store(T* __restrict__ p, const float (&acc)[N], float scale) {
   float x[N];
@@ -100,18 +95,275 @@ __device__ __forceinline__ void emb_store(T* __restrict__ p, const float (&acc)[
   store_vec<T, N>(p, x);
 }
 
-__global__ __launch_bounds__(EMB_THREADS) void embed_keys_kernel(int64_t n, int64_t V, const void* __restrict__ ids,
-                                                                 int id_bytes, uint64_t* __restrict__ keys,
-                                                                 uint32_t* __restrict__ pos) {
-  const int64_t i = (int64_t)blockIdx.x * EMB_THREADS + threadIdx.x;
-  if (i >= n) return;
-  const int64_t id = emb_id(ids, id_bytes, i);
-  keys[i] = id >= 0 && id < V ? (uint64_t)id : (uint64_t)V;  // ids that select nothing sort behind all rows
-  pos[i] = (uint32_t)i;
+// ---- the table's zeros, in `shares` stretches of whole vectors (the first also has what lies before and behind them)
+struct EmbFill {
+  char* base;
+  int64_t bytes;
+  int32_t share, shares;
+};
+
+__device__ __forceinline__ void emb_fill(const EmbFill& f, int64_t block, int64_t blocks) {
+  const int64_t lead = (int64_t)((16u - ((uintptr_t)f.base & 15u)) & 15u), head = lead < f.bytes ? lead : f.bytes;
+  const int64_t vecs = (f.bytes - head) / 16;
+  const int64_t per = (vecs + f.shares - 1) / f.shares, v0 = f.share * per, v1 = v0 + per < vecs ? v0 + per : vecs;
+  uint4* body = reinterpret_cast<uint4*>(f.base + head);
+  for (int64_t v = v0 + block * blockDim.x + threadIdx.x; v < v1; v += blocks * blockDim.x) body[v] = make_uint4(0, 0, 0, 0);
+  if (f.share == 0 && block == 0) {
+    const int64_t tail = head + vecs * 16, i = (int64_t)threadIdx.x * 2;  // both are fewer than 8 pairs of bytes
+    if (i < head) *reinterpret_cast<uint16_t*>(f.base + i) = 0;
+    if (tail + i < f.bytes) *reinterpret_cast<uint16_t*>(f.base + tail + i) = 0;
+  }
 }
 
+// ---- stable sort of the ids with their positions
+__device__ __forceinline__ uint32_t emb_key(const void* ids, int id_bytes, int64_t i, int64_t V) {
+  const int64_t id = emb_id(ids, id_bytes, i);
+  return id >= 0 && id < V ? (uint32_t)id : (uint32_t)V;  // ids that select nothing sort behind all rows
+}
+
+// the lanes (of those that take part) with this lane's digit of `bits` bits
+__device__ __forceinline__ unsigned long long emb_peers(uint32_t d, int bits, bool valid) {
+  unsigned long long peers = __ballot(valid);
+  for (int b = 0; b < bits; ++b) {
+    const bool bit = (d >> b) & 1u;
+    const unsigned long long m = __ballot(bit);
+    peers &= bit ? m : ~m;
+  }
+  return peers;
+}
+
+// One digit of the items that a workgroup holds in registers, wave by wave in their order: cnt [waves][radix] gets each
+// wave's counts, and each item its rank among its wave's items of the same digit.
+template <int ITEMS>
+__device__ __forceinline__ void emb_rank(const uint32_t (&key)[ITEMS], int64_t wave_first, int64_t n, int shift, int bits,
+                                         uint32_t* __restrict__ cnt, uint32_t (&rank)[ITEMS]) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const bool valid = wave_first + i * 64 + lane < n;
+    const uint32_t d = (key[i] >> shift) & ((1u << bits) - 1u);
+    const unsigned long long peers = emb_peers(d, bits, valid);
+    const uint32_t before = (uint32_t)__popcll(peers & ((1ull << lane) - 1ull));
+    const uint32_t prev = cnt[d];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    if (valid && before == 0) cnt[d] = prev + (uint32_t)__popcll(peers);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    rank[i] = prev + before;
+  }
+}
+
+// exclusive sum over the workgroup's threads; `lds` has a word for each wave
+template <int THREADS> __device__ __forceinline__ uint32_t emb_scan(uint32_t v, uint32_t* lds) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t incl = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t t = __shfl_up(incl, o);
+    if (lane >= o) incl += t;
+  }
+  if (lane == 63) lds[wave] = incl;
+  __syncthreads();
+  uint32_t before = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w)
+    if (w < wave) before += lds[w];
+  __syncthreads();
+  return before + incl - v;
+}
+
+// Workgroup 0 sorts up to 1024 ITEMS ids in LDS, digits of at most 8 bits; the others fill.
+template <int ITEMS>
+__global__ __launch_bounds__(EMB_SORT1_THREADS) void embed_sort1_kernel(int n, int64_t V, int bits,
+                                                                        const void* __restrict__ ids, int id_bytes,
+                                                                        uint32_t* __restrict__ keys_out,
+                                                                        uint32_t* __restrict__ pos_out, EmbFill fill) {
+  if (blockIdx.x > 0) {
+    emb_fill(fill, blockIdx.x - 1, gridDim.x - 1);
+    return;
+  }
+  constexpr int WAVES = EMB_SORT1_THREADS / 64, RADIX = 256;
+  __shared__ uint32_t cnt[WAVES][RADIX];
+  __shared__ uint32_t keys[ITEMS * EMB_SORT1_THREADS];
+  __shared__ uint16_t poss[ITEMS * EMB_SORT1_THREADS];
+  __shared__ uint32_t wsum[WAVES];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, first = wave * 64 * ITEMS;
+  const int passes = (bits + 7) / 8, per = (bits + passes - 1) / passes;
+  uint32_t key[ITEMS], rank[ITEMS];
+  uint16_t pos[ITEMS];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int at = first + i * 64 + lane;
+    key[i] = at < n ? emb_key(ids, id_bytes, at, V) : 0;
+    pos[i] = (uint16_t)at;
+  }
+  for (int p = 0; p < passes; ++p) {
+    for (int d = threadIdx.x; d < WAVES * RADIX; d += EMB_SORT1_THREADS) (&cnt[0][0])[d] = 0;
+    __syncthreads();
+    const int shift = p * per, width = bits - shift < per ? bits - shift : per;
+    emb_rank<ITEMS>(key, first, n, shift, width, cnt[wave], rank);
+    __syncthreads();
+    uint32_t total = 0;
+    if (threadIdx.x < RADIX)
+      for (int w = 0; w < WAVES; ++w) total += cnt[w][threadIdx.x];
+    uint32_t run = emb_scan<EMB_SORT1_THREADS>(total, wsum);
+    if (threadIdx.x < RADIX)
+      for (int w = 0; w < WAVES; ++w) {
+        const uint32_t c = cnt[w][threadIdx.x];
+        cnt[w][threadIdx.x] = run;
+        run += c;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i)
+      if (first + i * 64 + lane < n) {
+        const uint32_t to = cnt[wave][(key[i] >> shift) & ((1u << width) - 1u)] + rank[i];
+        if (p == passes - 1) {
+          keys_out[to] = key[i];
+          pos_out[to] = pos[i];
+        } else {
+          keys[to] = key[i];
+          poss[to] = pos[i];
+        }
+      }
+    __syncthreads();
+    if (p < passes - 1) {
+#pragma unroll
+      for (int i = 0; i < ITEMS; ++i) {
+        const int at = first + i * 64 + lane;
+        key[i] = at < n ? keys[at] : 0;
+        pos[i] = at < n ? poss[at] : 0;
+      }
+    }
+  }
+}
+
+// One digit of the radix sort: the digits' counts per workgroup (digit by digit), their sums over the workgroups before,
+// and the scatter.  `keys` NULL: the first digit, straight from the ids.  Workgroups from `blocks` on fill.
+struct EmbDigit {
+  int64_t n, V;
+  const void* ids;
+  int32_t id_bytes, shift, bits, blocks;
+  const uint32_t *keys, *pos;
+  uint32_t *keys_out, *pos_out;
+  uint32_t *table, *totals;  // [radix][blocks], [radix]
+  EmbFill fill;
+};
+
+__device__ __forceinline__ void emb_load_items(const EmbDigit& s, int64_t first, uint32_t (&key)[EMB_ITEMS]) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < EMB_ITEMS; ++i) {
+    const int64_t at = first + i * 64 + lane;
+    key[i] = at < s.n ? (s.keys ? s.keys[at] : emb_key(s.ids, s.id_bytes, at, s.V)) : 0;
+  }
+}
+
+__global__ __launch_bounds__(EMB_THREADS) void embed_hist_kernel(EmbDigit s) {
+  if ((int)blockIdx.x >= s.blocks) {
+    emb_fill(s.fill, blockIdx.x - s.blocks, gridDim.x - s.blocks);
+    return;
+  }
+  __shared__ uint32_t hist[EMB_RADIX];
+  for (int d = threadIdx.x; d < EMB_RADIX; d += EMB_THREADS) hist[d] = 0;
+  __syncthreads();
+  const int lane = threadIdx.x & 63;
+  const int64_t first = (int64_t)blockIdx.x * EMB_TILE + (threadIdx.x >> 6) * (64 * EMB_ITEMS);
+  uint32_t key[EMB_ITEMS];
+  emb_load_items(s, first, key);
+#pragma unroll
+  for (int i = 0; i < EMB_ITEMS; ++i) {  // one addition per digit that a wave holds: grouped ids would queue up
+    const bool valid = first + i * 64 + lane < s.n;
+    const uint32_t d = (key[i] >> s.shift) & ((1u << s.bits) - 1u);
+    const unsigned long long peers = emb_peers(d, s.bits, valid);
+    if (valid && (peers & ((1ull << lane) - 1ull)) == 0) atomicAdd(&hist[d], (uint32_t)__popcll(peers));
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < 1 << s.bits; d += EMB_THREADS) s.table[(int64_t)d * s.blocks + blockIdx.x] = hist[d];
+}
+
+// a wave per digit
+__global__ __launch_bounds__(EMB_THREADS) void embed_digit_sums_kernel(EmbDigit s) {
+  const int own = (1 << s.bits) / (EMB_THREADS / 64) + ((1 << s.bits) % (EMB_THREADS / 64) ? 1 : 0);
+  if ((int)blockIdx.x >= own) {
+    emb_fill(s.fill, blockIdx.x - own, gridDim.x - own);
+    return;
+  }
+  const int lane = threadIdx.x & 63, d = blockIdx.x * (EMB_THREADS / 64) + (threadIdx.x >> 6);
+  if (d >= 1 << s.bits) return;
+  uint32_t* row = s.table + (int64_t)d * s.blocks;
+  uint32_t run = 0;
+  for (int c0 = 0; c0 < s.blocks; c0 += 64) {
+    const int c = c0 + lane;
+    const uint32_t v = c < s.blocks ? row[c] : 0u;
+    uint32_t incl = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t t = __shfl_up(incl, o);
+      if (lane >= o) incl += t;
+    }
+    if (c < s.blocks) row[c] = run + incl - v;
+    run += __shfl(incl, 63);
+  }
+  if (lane == 0) s.totals[d] = run;
+}
+
+__global__ __launch_bounds__(EMB_THREADS) void embed_scatter_kernel(EmbDigit s) {
+  if ((int)blockIdx.x >= s.blocks) {
+    emb_fill(s.fill, blockIdx.x - s.blocks, gridDim.x - s.blocks);
+    return;
+  }
+  constexpr int WAVES = EMB_THREADS / 64, PER = EMB_RADIX / EMB_THREADS;
+  __shared__ uint32_t cnt[WAVES][EMB_RADIX];
+  __shared__ uint32_t start[EMB_RADIX];
+  __shared__ uint32_t wsum[WAVES];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, radix = 1 << s.bits;
+  const int64_t first = (int64_t)blockIdx.x * EMB_TILE + wave * (64 * EMB_ITEMS);
+  for (int d = threadIdx.x; d < WAVES * EMB_RADIX; d += EMB_THREADS) (&cnt[0][0])[d] = 0;
+  uint32_t key[EMB_ITEMS], pos[EMB_ITEMS], rank[EMB_ITEMS], t[PER], sum = 0;
+  emb_load_items(s, first, key);
+#pragma unroll
+  for (int i = 0; i < EMB_ITEMS; ++i) {
+    const int64_t at = first + i * 64 + lane;
+    pos[i] = s.pos && at < s.n ? s.pos[at] : (uint32_t)at;
+  }
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int d = threadIdx.x * PER + k;
+    t[k] = d < radix ? s.totals[d] : 0u;
+    sum += t[k];
+  }
+  uint32_t run = emb_scan<EMB_THREADS>(sum, wsum);  // (its barriers also stand behind the zeros of cnt)
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    start[threadIdx.x * PER + k] = run;
+    run += t[k];
+  }
+  emb_rank<EMB_ITEMS>(key, first, s.n, s.shift, s.bits, cnt[wave], rank);
+  __syncthreads();
+  for (int d = threadIdx.x; d < radix; d += EMB_THREADS) {
+    uint32_t at = start[d] + s.table[(int64_t)d * s.blocks + blockIdx.x];
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const uint32_t c = cnt[w][d];
+      cnt[w][d] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < EMB_ITEMS; ++i)
+    if (first + i * 64 + lane < s.n) {
+      const uint32_t to = cnt[wave][(key[i] >> s.shift) & (uint32_t)(radix - 1)] + rank[i];
+      s.keys_out[to] = key[i];
+      s.pos_out[to] = pos[i];
+    }
+}
+
+// ---- sums of the runs
 // first index in [lo, hi) with keys >= v
-__device__ __forceinline__ int64_t emb_lower(const uint64_t* __restrict__ keys, int64_t lo, int64_t hi, uint64_t v) {
+__device__ __forceinline__ int64_t emb_lower(const uint32_t* keys, int64_t lo, int64_t hi, uint32_t v) {
   while (lo < hi) {
     const int64_t mid = (lo + hi) >> 1;
     if (keys[mid] < v) lo = mid + 1; else hi = mid;
@@ -119,110 +371,140 @@ __device__ __forceinline__ int64_t emb_lower(const uint64_t* __restrict__ keys, 
   return lo;
 }
 
+// A group of G lanes takes the P sorted entries [i0, i1); its workgroup has their keys in LDS, with P more on both sides.
+// partial [pieces][2][D] fp32: what lies in the piece of the long run that started before it (slot 0), and of the long
+// run that starts in it (slot 1; there is one at most, and it goes on behind the piece).
 template <typename T, int N>
-__global__ __launch_bounds__(EMB_THREADS) void embed_rows_kernel(EmbShape sh, const uint64_t* __restrict__ keys,
+__global__ __launch_bounds__(EMB_THREADS) void embed_runs_kernel(EmbShape sh, const uint32_t* __restrict__ keys,
                                                                  const uint32_t* __restrict__ pos,
-                                                                 const T* __restrict__ v_out, T* __restrict__ v_table) {
-  __shared__ int64_t start[EMB_ROWS_MAX + 1];
-  const int64_t v0 = (int64_t)blockIdx.x * sh.rows_per;
-  const int rows = (int)(sh.V - v0 < sh.rows_per ? sh.V - v0 : sh.rows_per);
-  for (int r = threadIdx.x; r <= rows; r += EMB_THREADS) start[r] = emb_lower(keys, 0, sh.n, (uint64_t)(v0 + r));
+                                                                 const T* __restrict__ v_out, float* __restrict__ partial,
+                                                                 T* __restrict__ v_table) {
+  extern __shared__ uint32_t lds[];
+  const int P = sh.piece, groups = EMB_THREADS / sh.G, span = groups * P;
+  const int64_t w0 = (int64_t)blockIdx.x * span;
+  uint32_t* lkey = lds;               // entries [w0 - P, w0 + span + P]
+  uint32_t* lpos = lds + span + 2 * P + 1;  // entries [w0, w0 + span + P)
+  for (int l = threadIdx.x; l < span + 2 * P + 1; l += EMB_THREADS) {
+    const int64_t e = w0 - P + l;
+    lkey[l] = e < 0 ? 0xfffffffeu : e < sh.n ? keys[e] : 0xffffffffu;  // neither is a key
+  }
+  for (int l = threadIdx.x; l < span + P; l += EMB_THREADS) lpos[l] = w0 + l < sh.n ? pos[w0 + l] : 0u;
   __syncthreads();
-  const int g = threadIdx.x / sh.G, groups = EMB_THREADS / sh.G;
+  const int g = threadIdx.x / sh.G;
   const int64_t vec = (int64_t)blockIdx.y * sh.G + (threadIdx.x & (sh.G - 1));
-  if (vec >= sh.vpr) return;
-  for (int r = g; r < rows; r += groups) {
-    const int64_t s = start[r], e = start[r + 1];
-    if (e - s > EMB_LONG) continue;
-    float acc[N];
-#pragma unroll
-    for (int k = 0; k < N; ++k) acc[k] = 0.f;
-    emb_sum<T, N>(acc, pos, s, e, v_out, sh.gs, vec * N);
-    emb_store<T, N>(v_table + (v0 + r) * sh.vpr * N + vec * N, acc, sh.scale);
-  }
-}
-
-// The run of the key at `i`, known to start within EMB_LONG before it or to be long: true if it has more than EMB_LONG
-// entries.  `s` gets its start where that lies in (i - EMB_LONG, i].
-__device__ __forceinline__ bool emb_long(const uint64_t* __restrict__ keys, int64_t n, int64_t i, int64_t& s) {
-  const uint64_t k = keys[i];
-  if (i >= EMB_LONG && keys[i - EMB_LONG] == k) { s = -1; return true; }
-  s = emb_lower(keys, i >= EMB_LONG ? i - EMB_LONG + 1 : 0, i, k);
-  return s + EMB_LONG < n && keys[s + EMB_LONG] == k;
-}
-
-// partial [pieces][2][D] fp32: what of the long run that holds the piece's first entry (slot 0), and of the one that
-// holds its last entry where that is another (slot 1), lies in the piece
-template <typename T, int N>
-__global__ __launch_bounds__(EMB_THREADS) void embed_pieces_kernel(EmbShape sh, const uint64_t* __restrict__ keys,
-                                                                   const uint32_t* __restrict__ pos,
-                                                                   const T* __restrict__ v_out, float* __restrict__ partial) {
-  const int64_t p = (int64_t)blockIdx.x * (EMB_THREADS / sh.G) + threadIdx.x / sh.G;
-  const int64_t i0 = p * EMB_LONG;
-  const int64_t vec = (int64_t)blockIdx.y * sh.G + (threadIdx.x & (sh.G - 1));
+  const uint32_t* key = lkey + P + g * P;  // key[0]: the piece's first entry
+  const uint32_t* at = lpos + g * P;
+  const int64_t i0 = w0 + (int64_t)g * P;
   if (i0 >= sh.n || vec >= sh.vpr) return;
-  const int64_t i1 = i0 + EMB_LONG < sh.n ? i0 + EMB_LONG : sh.n;
-  const int64_t D = sh.vpr * N;
-  const uint64_t k0 = keys[i0], k1 = keys[i1 - 1];
-  int64_t s;
-  if (k0 < (uint64_t)sh.V && emb_long(keys, sh.n, i0, s)) {
-    const int64_t e = k1 == k0 ? i1 : emb_lower(keys, i0, i1, k0 + 1);
-    float acc[N];
-#pragma unroll
-    for (int k = 0; k < N; ++k) acc[k] = 0.f;
-    emb_sum<T, N>(acc, pos, i0, e, v_out, sh.gs, vec * N);
-    float* dst = partial + (2 * p) * D + vec * N;
-#pragma unroll
-    for (int k = 0; k < N; ++k) dst[k] = acc[k];
-  }
-  if (k1 != k0 && k1 < (uint64_t)sh.V && emb_long(keys, sh.n, i1 - 1, s)) {  // starts inside the piece: s is its start
-    float acc[N];
-#pragma unroll
-    for (int k = 0; k < N; ++k) acc[k] = 0.f;
-    emb_sum<T, N>(acc, pos, s, i1, v_out, sh.gs, vec * N);
-    float* dst = partial + (2 * p + 1) * D + vec * N;
-#pragma unroll
-    for (int k = 0; k < N; ++k) dst[k] = acc[k];
-  }
-}
+  const int i1 = sh.n - i0 < P ? (int)(sh.n - i0) : P;
+  const uint32_t V = (uint32_t)sh.V;
 
-// One workgroup per piece and column tile: the one in whose piece a long run starts adds the run's pieces, the groups of
-// the workgroup in turn, and joins the groups in LDS.
-template <typename T, int N>
-__global__ __launch_bounds__(EMB_THREADS) void embed_join_kernel(EmbShape sh, const uint64_t* __restrict__ keys,
-                                                                 const float* __restrict__ partial, T* __restrict__ v_table) {
-  const int64_t p = blockIdx.x;
-  const int64_t i0 = p * EMB_LONG;
-  const int64_t i1 = i0 + EMB_LONG < sh.n ? i0 + EMB_LONG : sh.n;
-  const uint64_t key = keys[i1 - 1];
-  if (key >= (uint64_t)sh.V || i1 >= sh.n || keys[i1] != key) return;  // a long run that starts here goes on behind the piece
-  if (i0 > 0 && keys[i0 - 1] == key) return;                           // started before
-  const int64_t s = emb_lower(keys, i0, i1, key);
-  if (s + EMB_LONG >= sh.n || keys[s + EMB_LONG] != key) return;
-  const int64_t e = emb_lower(keys, s + EMB_LONG, sh.n, key + 1);
-  const int64_t last = (e - 1) / EMB_LONG;  // the piece of its last entry
-  const int g = threadIdx.x / sh.G, groups = EMB_THREADS / sh.G;
-  const int64_t vec = (int64_t)blockIdx.y * sh.G + (threadIdx.x & (sh.G - 1));
-  const int64_t D = sh.vpr * N;
+  int a = 0;            // first entry to add
+  bool before = false;  // ... which belongs to a long run that started before the piece
+  if (key[-1] == key[0]) {
+    const uint32_t k = key[0];
+    const int s = key[-P] == k ? -P : (int)emb_lower(key, -P + 1, 0, k);
+    before = s == -P || key[s + P] == k;
+    if (!before) a = (int)emb_lower(key, 0, i1, k + 1);  // a short run: the group where it starts has it
+  }
+  int b = i1;  // behind the last entry to add
+  if (a < i1 && key[i1] == key[i1 - 1]) {
+    const uint32_t k = key[i1 - 1];
+    const int s = (int)emb_lower(key, a, i1, k);
+    if (!(before && s == 0) && key[s + P] != k) b = (int)emb_lower(key, i1, i1 + P, k + 1);  // a short run that starts here
+  }
+  const int64_t D = sh.vpr * N, col = vec * N, p = i0 / P;
   float acc[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) acc[k] = 0.f;
-  if (vec < sh.vpr) {
-    for (int64_t q = p + g; q <= last; q += groups) {
-      const float* src = partial + (2 * q + (q == p && s != i0 ? 1 : 0)) * D + vec * N;
+  int s = a;  // start of the run that is being added
+  for (int i = a; i < b; i += 4) {
+    if (key[i] >= V) break;  // nothing but ids that select nothing from here on
+    float x[4][N];
 #pragma unroll
-      for (int k = 0; k < N; ++k) acc[k] += src[k];
+    for (int u = 0; u < 4; ++u) {
+      const int e = i + u < b ? i + u : b - 1;
+      load_vec<T, N>(v_out + (int64_t)at[e] * sh.gs + col, x[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int e = i + u;
+      if (e < b && key[e] < V) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] += x[u][k];
+        if (e + 1 == b || key[e + 1] != key[e]) {
+          if (before || key[s + P] == key[s]) {
+            float* to = partial + (2 * p + (before ? 0 : 1)) * D + col;
+#pragma unroll
+            for (int k = 0; k < N; ++k) to[k] = acc[k];
+          } else {
+            emb_store<T, N>(v_table + (int64_t)key[e] * D + col, acc, sh.scale);
+          }
+#pragma unroll
+          for (int k = 0; k < N; ++k) acc[k] = 0.f;
+          before = false;
+          s = e + 1;
+        }
+      }
     }
   }
-  __shared__ float lds[EMB_THREADS * N];
-#pragma unroll
-  for (int k = 0; k < N; ++k) lds[threadIdx.x * N + k] = acc[k];
+}
+
+// A workgroup looks at EMB_JOIN_PIECES pieces; for each in which a long run starts it adds the run's pieces, its groups in
+// turn, and joins the groups in LDS, in their order.
+template <typename T, int N>
+__global__ __launch_bounds__(EMB_JOIN_THREADS) void embed_join_kernel(EmbShape sh, const uint32_t* __restrict__ keys,
+                                                                      const float* __restrict__ partial,
+                                                                      T* __restrict__ v_table) {
+  __shared__ float lds[EMB_JOIN_THREADS * N];
+  __shared__ int64_t start[EMB_JOIN_PIECES];  // of the long run that starts in the piece, -1: none does
+  const int P = sh.piece;
+  const int64_t p0 = (int64_t)blockIdx.x * EMB_JOIN_PIECES;
+  if (threadIdx.x < EMB_JOIN_PIECES) {
+    const int64_t i0 = (p0 + threadIdx.x) * P, i1 = i0 + P;
+    int64_t s = -1;
+    if (i1 < sh.n) {  // it goes on behind the piece
+      const uint32_t k = keys[i1 - 1];
+      if (k < (uint32_t)sh.V && keys[i1] == k && !(i0 > 0 && keys[i0 - 1] == k)) {
+        s = emb_lower(keys, i0, i1, k);
+        if (!(s + P < sh.n && keys[s + P] == k)) s = -1;
+      }
+    }
+    start[threadIdx.x] = s;
+  }
   __syncthreads();
-  if (g != 0 || vec >= sh.vpr) return;
-  for (int h = 1; h < groups; ++h)
+  const int g = threadIdx.x / sh.G, groups = EMB_JOIN_THREADS / sh.G;
+  const int64_t vec = (int64_t)blockIdx.y * sh.G + (threadIdx.x & (sh.G - 1));
+  const int64_t D = sh.vpr * N;
+  for (int q = 0; q < EMB_JOIN_PIECES; ++q) {
+    const int64_t s = start[q];
+    if (s < 0) continue;
+    const uint32_t key = keys[s];
+    const int64_t e = emb_lower(keys, s + P, sh.n, key + 1), last = (e - 1) / P;  // the piece of its last entry
+    float acc[N];
 #pragma unroll
-    for (int k = 0; k < N; ++k) acc[k] += lds[(h * sh.G + threadIdx.x) * N + k];
-  emb_store<T, N>(v_table + (int64_t)key * D + vec * N, acc, sh.scale);
+    for (int k = 0; k < N; ++k) acc[k] = 0.f;
+    if (vec < sh.vpr) {
+#pragma unroll 4
+      for (int64_t r = p0 + q + g; r <= last; r += groups) {
+        const float* src = partial + (2 * r + (r == p0 + q ? 1 : 0)) * D + vec * N;
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] += src[k];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) lds[k * EMB_JOIN_THREADS + threadIdx.x] = acc[k];
+    __syncthreads();
+    if (g == 0 && vec < sh.vpr) {
+      const int64_t full = last - (p0 + q) + 1;
+      const int have = full < groups ? (int)full : groups;
+      for (int h = 1; h < have; ++h)
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] += lds[k * EMB_JOIN_THREADS + h * sh.G + threadIdx.x];
+      emb_store<T, N>(v_table + (int64_t)key * D + vec * N, acc, sh.scale);
+    }
+    __syncthreads();
+  }
 }
 
 // Few ids: one launch.  The workgroup lists, in order, the ids that fall among its rows; each group adds those of its row.
@@ -290,21 +572,77 @@ static int emb_bits(int64_t V) {
 static int64_t emb_round(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
 struct EmbWorkspace {
-  int64_t keys, pos, keys_b, pos_b, sort, sort_bytes, partial, total;
+  int64_t keys, pos, keys_b, pos_b, table, totals, partial, total;
 };
+
+static int emb_piece(int64_t n) { return n <= 65536 ? 16 : 64; }  // enough pieces for the card, then fewer long runs
 
 static EmbWorkspace emb_workspace(int64_t n, int64_t V, int64_t D) {
   EmbWorkspace w = {};
   if (n <= EMB_DIRECT) return w;
-  w.keys = 0;
-  w.pos = w.keys + emb_round(8 * n);
-  w.keys_b = w.pos + emb_round(4 * n);
-  w.pos_b = w.keys_b + emb_round(8 * n);
-  w.sort = w.pos_b + emb_round(4 * n);
-  w.sort_bytes = gs_radix_sort_workspace_bytes(n);
-  w.partial = w.sort + emb_round(w.sort_bytes);
-  w.total = w.partial + 8 * D * ceil_div(n, EMB_LONG);
+  const int64_t list = emb_round(4 * n), blocks = ceil_div(n, EMB_TILE);
+  w.pos = w.keys + list;
+  w.keys_b = w.pos + list;
+  w.pos_b = w.keys_b + list;
+  w.table = w.pos_b + list;
+  w.totals = w.table + emb_round(4 * EMB_RADIX * blocks);
+  w.partial = w.totals + emb_round(4 * EMB_RADIX);
+  w.total = w.partial + 8 * D * ceil_div(n, emb_piece(n));
   return w;
+}
+
+// workgroups that fill one share of the table: 16 KiB each, at most eight on a CU
+static unsigned emb_fill_blocks(const EmbFill& f, int threads) {
+  const int64_t b = ceil_div(f.bytes / f.shares, (int64_t)threads * 64);
+  return (unsigned)std::min<int64_t>(std::max<int64_t>(b, 1), 2048 * 256 / threads);
+}
+
+// sorts the ids and zeroes the table; `w` says which of the two pairs of lists has the result
+static int emb_sort(int64_t n, int64_t V, const void* ids, int32_t id_bytes, char* ws, const EmbWorkspace& w, void* v_table,
+                    int64_t table_bytes, const uint32_t** keys, const uint32_t** pos, hipStream_t s) {
+  const int bits = emb_bits(V);
+  EmbFill fill{(char*)v_table, table_bytes, 0, 1};
+  uint32_t *ka = (uint32_t*)(ws + w.keys), *pa = (uint32_t*)(ws + w.pos);
+  uint32_t *kb = (uint32_t*)(ws + w.keys_b), *pb = (uint32_t*)(ws + w.pos_b);
+  if (n <= EMB_SORT1) {
+    const dim3 grid(1 + emb_fill_blocks(fill, EMB_SORT1_THREADS)), block(EMB_SORT1_THREADS);
+    if (n <= 4 * EMB_SORT1_THREADS)
+      hipLaunchKernelGGL(embed_sort1_kernel<4>, grid, block, 0, s, (int)n, V, bits, ids, id_bytes, ka, pa, fill);
+    else
+      hipLaunchKernelGGL(embed_sort1_kernel<16>, grid, block, 0, s, (int)n, V, bits, ids, id_bytes, ka, pa, fill);
+    GS_CHECK_LAUNCH();
+    *keys = ka;
+    *pos = pa;
+    return GS_OK;
+  }
+  const int passes = (bits + EMB_RADIX_BITS - 1) / EMB_RADIX_BITS, per = (bits + passes - 1) / passes;
+  EmbDigit d{};
+  d.n = n; d.V = V; d.ids = ids; d.id_bytes = id_bytes;
+  d.blocks = (int32_t)ceil_div(n, EMB_TILE);
+  d.table = (uint32_t*)(ws + w.table);
+  d.totals = (uint32_t*)(ws + w.totals);
+  fill.shares = 3 * passes;
+  const unsigned more = emb_fill_blocks(fill, EMB_THREADS);
+  const dim3 block(EMB_THREADS);
+  for (int p = 0; p < passes; ++p) {
+    d.shift = p * per;
+    d.bits = std::min(per, bits - d.shift);
+    d.keys = p ? (p & 1 ? ka : kb) : nullptr;
+    d.pos = p ? (p & 1 ? pa : pb) : nullptr;
+    d.keys_out = p & 1 ? kb : ka;
+    d.pos_out = p & 1 ? pb : pa;
+    d.fill = fill;
+    d.fill.share = 3 * p;
+    hipLaunchKernelGGL(embed_hist_kernel, dim3(d.blocks + more), block, 0, s, d);
+    d.fill.share = 3 * p + 1;
+    hipLaunchKernelGGL(embed_digit_sums_kernel, dim3((unsigned)ceil_div(1 << d.bits, EMB_THREADS / 64) + more), block, 0, s, d);
+    d.fill.share = 3 * p + 2;
+    hipLaunchKernelGGL(embed_scatter_kernel, dim3(d.blocks + more), block, 0, s, d);
+    GS_CHECK_LAUNCH();
+  }
+  *keys = d.keys_out;
+  *pos = d.pos_out;
+  return GS_OK;
 }
 
 }  // namespace gs
@@ -366,45 +704,34 @@ extern "C" int gs_embedding_bwd(int64_t n, int64_t V, int64_t D, int32_t dtype, 
   while (sh.G < 64 && sh.G < sh.vpr) sh.G <<= 1;
   const int64_t tiles = ceil_div(sh.vpr, sh.G);
   if (tiles > 65535) return GS_ERR_UNSUPPORTED;  // rows above 4M vectors
-  // enough workgroups for 256 CUs first, then more rows each
-  const int groups = EMB_THREADS / sh.G;
-  int64_t per = ceil_div(V * tiles, 2048);
-  per = per < groups ? groups : per;
-  sh.rows_per = (int)(per < EMB_ROWS_MAX ? per : EMB_ROWS_MAX);
-  const int64_t row_blocks = ceil_div(V, sh.rows_per);
-  const dim3 row_grid((unsigned)row_blocks, (unsigned)tiles);
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     return with_vec(size, N, [&](auto nv) {
       constexpr int NV = decltype(nv)::value;
       if constexpr (NV * (int)sizeof(T) <= 16) {
         if (n <= EMB_DIRECT) {
-          hipLaunchKernelGGL((embed_direct_kernel<T, NV>), row_grid, dim3(EMB_THREADS), 0, s, sh, ids, id_bytes,
-                             (const T*)v_out, (T*)v_table);
+          // enough workgroups for 256 CUs first, then more rows each
+          const int64_t per = std::max<int64_t>(ceil_div(V * tiles, 2048), EMB_THREADS / sh.G);
+          sh.rows_per = (int)std::min<int64_t>(per, EMB_ROWS_MAX);
+          hipLaunchKernelGGL((embed_direct_kernel<T, NV>), dim3((unsigned)ceil_div(V, sh.rows_per), (unsigned)tiles),
+                             dim3(EMB_THREADS), 0, s, sh, ids, id_bytes, (const T*)v_out, (T*)v_table);
           GS_CHECK_LAUNCH();
           return GS_OK;
         }
-        char* b = (char*)workspace;
-        uint64_t* keys = (uint64_t*)(b + w.keys);
-        uint32_t* pos = (uint32_t*)(b + w.pos);
-        hipLaunchKernelGGL(embed_keys_kernel, dim3((unsigned)ceil_div(n, EMB_THREADS)), dim3(EMB_THREADS), 0, s, n, V, ids,
-                           id_bytes, keys, pos);
-        GS_CHECK_LAUNCH();
-        int32_t in_b = 0;
-        const int st = gs_radix_sort_pairs_u64_u32_bits(n, 0, emb_bits(V), keys, pos, (uint64_t*)(b + w.keys_b),
-                                                        (uint32_t*)(b + w.pos_b), b + w.sort, w.sort_bytes, &in_b, stream);
+        const uint32_t *keys, *pos;
+        const int st = emb_sort(n, V, ids, id_bytes, (char*)workspace, w, v_table, V * D * size, &keys, &pos, s);
         if (st != GS_OK) return st;
-        if (in_b) { keys = (uint64_t*)(b + w.keys_b); pos = (uint32_t*)(b + w.pos_b); }
-        hipLaunchKernelGGL((embed_rows_kernel<T, NV>), row_grid, dim3(EMB_THREADS), 0, s, sh, keys, pos, (const T*)v_out,
+        sh.G = std::max(sh.G, 4);  // (keeps a workgroup's share of the sorted ids within 32 KiB of LDS)
+        sh.piece = emb_piece(n);
+        float* partial = (float*)((char*)workspace + w.partial);
+        const int64_t pieces = ceil_div(n, sh.piece);
+        const int span = EMB_THREADS / sh.G * sh.piece;
+        hipLaunchKernelGGL((embed_runs_kernel<T, NV>), dim3((unsigned)ceil_div(n, span), (unsigned)tiles), dim3(EMB_THREADS),
+                           (2 * span + 3 * sh.piece + 1) * sizeof(uint32_t), s, sh, keys, pos, (const T*)v_out, partial,
                            (T*)v_table);
         GS_CHECK_LAUNCH();
-        float* partial = (float*)(b + w.partial);
-        const int64_t pieces = ceil_div(n, EMB_LONG);
-        hipLaunchKernelGGL((embed_pieces_kernel<T, NV>), dim3((unsigned)ceil_div(pieces, groups), (unsigned)tiles),
-                           dim3(EMB_THREADS), 0, s, sh, keys, pos, (const T*)v_out, partial);
-        GS_CHECK_LAUNCH();
-        hipLaunchKernelGGL((embed_join_kernel<T, NV>), dim3((unsigned)pieces, (unsigned)tiles), dim3(EMB_THREADS), 0, s, sh,
-                           keys, partial, (T*)v_table);
+        hipLaunchKernelGGL((embed_join_kernel<T, NV>), dim3((unsigned)ceil_div(pieces, EMB_JOIN_PIECES), (unsigned)tiles),
+                           dim3(EMB_JOIN_THREADS), 0, s, sh, keys, partial, (T*)v_table);
         GS_CHECK_LAUNCH();
         return GS_OK;
       }
