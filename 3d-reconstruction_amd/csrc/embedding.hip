@@ -11,7 +11,8 @@
 //      what lies in its piece.
 //   3. embed_join_kernel adds the pieces of each long run.
 // Sums are held in fp32, taken in an order that the ids alone fix (no float atomics), and rounded once at the end.
-// Up to EMB_DIRECT ids need no sort: each workgroup picks the ids that fall among its rows of the table.
+// Up to EMB_DIRECT ids need no sort: each workgroup picks the ids that fall among its rows of the table.  Nor does a table
+// of up to EMB_FEW rows, however many ids: it is added up in LDS.
 #include <algorithm>
 #include <type_traits>
 
@@ -20,7 +21,9 @@
 namespace gs {
 
 constexpr int EMB_THREADS = 256;
+constexpr int EMB_FLIGHT = 4;         // rows a thread of the lookup has in flight
 constexpr int EMB_DIRECT = 256;
+constexpr int EMB_FEW = 64;           // rows of a table that fits LDS once for each row a workgroup reads at a time
 constexpr int EMB_ROWS_MAX = 256;     // rows of the table per workgroup of the direct form
 constexpr int EMB_SORT1 = 16384;      // ids that one workgroup sorts in LDS
 constexpr int EMB_SORT1_THREADS = 1024;
@@ -30,6 +33,7 @@ constexpr int EMB_ITEMS = 8;          // ids per thread and launch of the radix 
 constexpr int EMB_TILE = EMB_THREADS * EMB_ITEMS;
 constexpr int EMB_JOIN_THREADS = 1024;
 constexpr int EMB_JOIN_PIECES = 16;   // pieces that a workgroup of the join looks at
+constexpr int EMB_PIECE_MAX = 64;
 
 __device__ __forceinline__ int64_t emb_id(const void* ids, int id_bytes, int64_t i) {
   return id_bytes == 8 ? ((const int64_t*)ids)[i] : (int64_t)((const int32_t*)ids)[i];
@@ -46,25 +50,35 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_lookup_kernel(int64_t n, in
   for (int64_t r0 = (int64_t)blockIdx.x * rows_per; r0 < n; r0 += (int64_t)gridDim.x * rows_per) {
     const int64_t rows = n - r0 < rows_per ? n - r0 : rows_per;
     const int64_t total = rows * vpr;
-    for (int64_t f = threadIdx.x; f < total; f += EMB_THREADS) {
-      int64_t r, c;
-      if (rows_per == 1) {
-        r = 0; c = f;
-      } else {
-        r = vpr == 1 ? f : (int64_t)__umulhi((uint32_t)f, magic);
-        c = f - r * vpr;
-      }
-      const int64_t id = emb_id(ids, id_bytes, r0 + r);
-      float x[N];
-      if (id >= 0 && id < V) {
-        load_vec<T, N>(table + id * ts + c * N, x);
+    for (int64_t f0 = threadIdx.x; f0 < total; f0 += EMB_FLIGHT * EMB_THREADS) {
+      float x[EMB_FLIGHT][N];
+      int64_t id[EMB_FLIGHT], c[EMB_FLIGHT];
 #pragma unroll
-        for (int k = 0; k < N; ++k) x[k] *= scale;
-      } else {
-#pragma unroll
-        for (int k = 0; k < N; ++k) x[k] = 0.f;
+      for (int u = 0; u < EMB_FLIGHT; ++u) {
+        const int64_t f = f0 + u * EMB_THREADS < total ? f0 + u * EMB_THREADS : total - 1;
+        const int64_t r = rows_per == 1 ? 0 : vpr == 1 ? f : (int64_t)__umulhi((uint32_t)f, magic);
+        c[u] = (f - r * vpr) * N;
+        id[u] = emb_id(ids, id_bytes, r0 + r);
       }
-      store_vec<T, N>(out + ((r0 + r) * vpr + c) * N, x);
+#pragma unroll
+      for (int u = 0; u < EMB_FLIGHT; ++u) {
+        if (id[u] >= 0 && id[u] < V) {
+          load_vec<T, N>(table + id[u] * ts + c[u], x[u]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < N; ++k) x[u][k] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < EMB_FLIGHT; ++u) {
+        const int64_t f = f0 + u * EMB_THREADS;
+        if (f < total) {
+          const bool any = id[u] >= 0 && id[u] < V;  // (0 * scale is no zero for every scale)
+#pragma unroll
+          for (int k = 0; k < N; ++k) x[u][k] = any ? x[u][k] * scale : 0.f;
+          store_vec<T, N>(out + (r0 * vpr + f) * N, x[u]);
+        }
+      }
     }
   }
 }
@@ -450,25 +464,43 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_runs_kernel(EmbShape sh, co
   }
 }
 
+// emb_lower by a whole wave: 64 probes at a time
+__device__ __forceinline__ int64_t emb_lower_wave(const uint32_t* __restrict__ keys, int64_t lo, int64_t hi, uint32_t v) {
+  const int lane = threadIdx.x & 63;
+  while (lo < hi) {
+    const int64_t step = (hi - lo + 63) / 64, at = lo + (lane + 1) * step - 1;  // the last of the lane's stretch
+    const int64_t below = __popcll(__ballot(at < hi && keys[at < hi ? at : hi - 1] < v));
+    lo += below * step;
+    if (step == 1) break;
+    hi = lo + step - 1 < hi ? lo + step - 1 : hi;  // (its last entry is known not to be below)
+  }
+  return lo;
+}
+
 // A workgroup looks at EMB_JOIN_PIECES pieces; for each in which a long run starts it adds the run's pieces, its groups in
 // turn, and joins the groups in LDS, in their order.
 template <typename T, int N>
 __global__ __launch_bounds__(EMB_JOIN_THREADS) void embed_join_kernel(EmbShape sh, const uint32_t* __restrict__ keys,
                                                                       const float* __restrict__ partial,
                                                                       T* __restrict__ v_table) {
-  __shared__ float lds[EMB_JOIN_THREADS * N];
+  constexpr int MAX_KEYS = (EMB_JOIN_PIECES + 1) * EMB_PIECE_MAX + 1;
+  __shared__ float lds[EMB_JOIN_THREADS * N > MAX_KEYS ? EMB_JOIN_THREADS * N : MAX_KEYS];
   __shared__ int64_t start[EMB_JOIN_PIECES];  // of the long run that starts in the piece, -1: none does
   const int P = sh.piece;
   const int64_t p0 = (int64_t)blockIdx.x * EMB_JOIN_PIECES;
+  uint32_t* near = reinterpret_cast<uint32_t*>(lds);  // the keys from the one before the pieces on, and P behind them
+  for (int l = threadIdx.x; l <= (EMB_JOIN_PIECES + 1) * P; l += EMB_JOIN_THREADS) {
+    const int64_t e = p0 * P - 1 + l;
+    near[l] = e < 0 ? 0xfffffffeu : e < sh.n ? keys[e] : 0xffffffffu;  // neither is a key
+  }
+  __syncthreads();
   if (threadIdx.x < EMB_JOIN_PIECES) {
-    const int64_t i0 = (p0 + threadIdx.x) * P, i1 = i0 + P;
+    const uint32_t* key = near + 1 + threadIdx.x * P;  // key[0]: the piece's first entry
+    const uint32_t k = key[P - 1];
     int64_t s = -1;
-    if (i1 < sh.n) {  // it goes on behind the piece
-      const uint32_t k = keys[i1 - 1];
-      if (k < (uint32_t)sh.V && keys[i1] == k && !(i0 > 0 && keys[i0 - 1] == k)) {
-        s = emb_lower(keys, i0, i1, k);
-        if (!(s + P < sh.n && keys[s + P] == k)) s = -1;
-      }
+    if (k < (uint32_t)sh.V && key[P] == k && key[-1] != k) {  // it starts here and goes on behind the piece
+      const int at = (int)emb_lower(key, 0, P, k);
+      if (key[at + P] == k) s = (p0 + threadIdx.x) * P + at;
     }
     start[threadIdx.x] = s;
   }
@@ -480,7 +512,7 @@ __global__ __launch_bounds__(EMB_JOIN_THREADS) void embed_join_kernel(EmbShape s
     const int64_t s = start[q];
     if (s < 0) continue;
     const uint32_t key = keys[s];
-    const int64_t e = emb_lower(keys, s + P, sh.n, key + 1), last = (e - 1) / P;  // the piece of its last entry
+    const int64_t e = emb_lower_wave(keys, s + P, sh.n, key + 1), last = (e - 1) / P;  // the piece of its last entry
     float acc[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) acc[k] = 0.f;
@@ -504,6 +536,80 @@ __global__ __launch_bounds__(EMB_JOIN_THREADS) void embed_join_kernel(EmbShape s
       emb_store<T, N>(v_table + (int64_t)key * D + vec * N, acc, sh.scale);
     }
     __syncthreads();
+  }
+}
+
+// ---- few rows (V <= EMB_FEW): no sort.  256 threads read 256 values at a time, a column each (a row of D <= 128 columns
+// leaves room for several rows), and add them to a table in LDS that belongs to the thread's place among those rows: no
+// two threads meet in a word.  Equal ids in succession, the rule where Gaussians lie instance by instance, add up in a
+// register first.  The tables of a workgroup are added up, in their order, and embed_few_join_kernel adds the workgroups'.
+struct EmbFew {
+  int64_t n, per, gs;   // ids, ids of a workgroup, row stride of v_out
+  int32_t V, D, Dp;     // Dp: columns of a workgroup, a power of two
+};
+
+template <typename T>
+__global__ __launch_bounds__(EMB_THREADS) void embed_few_kernel(EmbFew sh, const void* __restrict__ ids, int id_bytes,
+                                                                const T* __restrict__ v_out, float* __restrict__ partial) {
+  extern __shared__ float tables[];  // [256 / Dp][V][Dp]
+  constexpr int U = 16;
+  const int S = EMB_THREADS / sh.Dp, c = threadIdx.x & (sh.Dp - 1), col = blockIdx.y * sh.Dp + c;
+  for (int e = threadIdx.x; e < sh.V * EMB_THREADS; e += EMB_THREADS) tables[e] = 0.f;
+  __syncthreads();
+  if (col < sh.D) {
+    float* mine = tables + threadIdx.x / sh.Dp * sh.V * sh.Dp + c;
+    const int64_t r0 = blockIdx.x * sh.per, r1 = r0 + sh.per < sh.n ? r0 + sh.per : sh.n;
+    int64_t last = -1;
+    float acc = 0.f;
+    for (int64_t r = r0 + threadIdx.x / sh.Dp; r < r1; r += (int64_t)U * S) {
+      int64_t id[U];
+      float x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t q = r + (int64_t)u * S < r1 ? r + (int64_t)u * S : r;
+        id[u] = emb_id(ids, id_bytes, q);
+        x[u] = (float)v_out[q * sh.gs + col];
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (r + (int64_t)u * S < r1) {
+          if (id[u] != last) {
+            if (last >= 0 && last < sh.V) mine[last * sh.Dp] += acc;
+            last = id[u];
+            acc = 0.f;
+          }
+          acc += x[u];
+        }
+    }
+    if (last >= 0 && last < sh.V) mine[last * sh.Dp] += acc;
+  }
+  __syncthreads();
+  const int size = sh.V * sh.Dp;
+  for (int e = threadIdx.x; e < size; e += EMB_THREADS) {
+    const int to = blockIdx.y * sh.Dp + (e & (sh.Dp - 1));
+    if (to >= sh.D) continue;
+    float sum = tables[e];
+    for (int k = 1; k < S; ++k) sum += tables[k * size + e];
+    partial[((int64_t)blockIdx.x * sh.V + e / sh.Dp) * sh.D + to] = sum;
+  }
+}
+
+// 32 words of the table at a time, 32 threads to each
+template <typename T>
+__global__ __launch_bounds__(1024) void embed_few_join_kernel(int words, int blocks, float scale,
+                                                              const float* __restrict__ partial, T* __restrict__ v_table) {
+  __shared__ float lds[32][33];
+  const int e = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
+  float acc = 0.f;
+  if (e < words) {
+#pragma unroll 8
+    for (int b = slice; b < blocks; b += 32) acc += partial[(int64_t)b * words + e];
+  }
+  lds[slice][threadIdx.x & 31] = acc;
+  __syncthreads();
+  if (slice == 0 && e < words) {
+    for (int k = 1; k < 32; ++k) acc += lds[k][threadIdx.x];
+    v_table[e] = (T)(acc * scale);
   }
 }
 
@@ -575,11 +681,25 @@ struct EmbWorkspace {
   int64_t keys, pos, keys_b, pos_b, table, totals, partial, total;
 };
 
-static int emb_piece(int64_t n) { return n <= 65536 ? 16 : 64; }  // enough pieces for the card, then fewer long runs
+// enough groups to fill the card first, then longer pieces: fewer partial sums of long runs
+static int emb_piece(int64_t n, int64_t D) { return n * D < ((int64_t)1 << 26) ? 16 : 64; }
+
+static bool emb_few(int64_t V, int64_t D) { return V <= EMB_FEW && D <= 65536; }
+
+// Workgroups of the form for few rows: two on each CU, each with eight times as many ids as the table has rows, so that
+// the tables cost little next to what they were added up from.
+static int64_t emb_few_blocks(int64_t n, int64_t V, int64_t D) {
+  const int64_t tiles = ceil_div(D, EMB_THREADS);
+  return std::max<int64_t>(1, std::min<int64_t>(ceil_div(512, tiles), n / (8 * V)));
+}
 
 static EmbWorkspace emb_workspace(int64_t n, int64_t V, int64_t D) {
   EmbWorkspace w = {};
   if (n <= EMB_DIRECT) return w;
+  if (emb_few(V, D)) {
+    w.total = 4 * V * D * emb_few_blocks(n, V, D);
+    return w;
+  }
   const int64_t list = emb_round(4 * n), blocks = ceil_div(n, EMB_TILE);
   w.pos = w.keys + list;
   w.keys_b = w.pos + list;
@@ -587,7 +707,7 @@ static EmbWorkspace emb_workspace(int64_t n, int64_t V, int64_t D) {
   w.table = w.pos_b + list;
   w.totals = w.table + emb_round(4 * EMB_RADIX * blocks);
   w.partial = w.totals + emb_round(4 * EMB_RADIX);
-  w.total = w.partial + 8 * D * ceil_div(n, emb_piece(n));
+  w.total = w.partial + 8 * D * ceil_div(n, emb_piece(n, D));
   return w;
 }
 
@@ -697,7 +817,7 @@ extern "C" int gs_embedding_bwd(int64_t n, int64_t V, int64_t D, int32_t dtype, 
   if (w.total > 0 && (!workspace || ((uintptr_t)workspace & 15))) return GS_ERR_INVALID_ARG;
   if (workspace_bytes < w.total) return GS_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
-  const int N = emb_vec(D, size, v_out_stride, v_out, v_table);
+  const int N = n > EMB_DIRECT && emb_few(V, D) ? 1 : emb_vec(D, size, v_out_stride, v_out, v_table);
   EmbShape sh;
   sh.n = n; sh.V = V; sh.vpr = D / N; sh.gs = v_out_stride; sh.scale = scale;
   sh.G = 1;
@@ -718,11 +838,28 @@ extern "C" int gs_embedding_bwd(int64_t n, int64_t V, int64_t D, int32_t dtype, 
           GS_CHECK_LAUNCH();
           return GS_OK;
         }
+        if (emb_few(V, D)) {
+          if constexpr (NV == 1) {
+            EmbFew few{n, 0, v_out_stride, (int32_t)V, (int32_t)D, 1};
+            while (few.Dp < EMB_THREADS && few.Dp < D) few.Dp <<= 1;
+            const int64_t blocks = emb_few_blocks(n, V, D);
+            few.per = ceil_div(n, blocks);
+            hipLaunchKernelGGL(embed_few_kernel<T>, dim3((unsigned)blocks, (unsigned)ceil_div(D, few.Dp)), dim3(EMB_THREADS),
+                               V * EMB_THREADS * sizeof(float), s, few, ids, id_bytes, (const T*)v_out, (float*)workspace);
+            GS_CHECK_LAUNCH();
+            const int words = (int)(V * D);
+            hipLaunchKernelGGL(embed_few_join_kernel<T>, dim3((unsigned)ceil_div(words, 32)), dim3(1024), 0, s, words,
+                               (int)blocks, scale, (const float*)workspace, (T*)v_table);
+            GS_CHECK_LAUNCH();
+            return GS_OK;
+          }
+          return GS_ERR_INVALID_ARG;
+        }
         const uint32_t *keys, *pos;
         const int st = emb_sort(n, V, ids, id_bytes, (char*)workspace, w, v_table, V * D * size, &keys, &pos, s);
         if (st != GS_OK) return st;
         sh.G = std::max(sh.G, 4);  // (keeps a workgroup's share of the sorted ids within 32 KiB of LDS)
-        sh.piece = emb_piece(n);
+        sh.piece = emb_piece(n, D);
         float* partial = (float*)((char*)workspace + w.partial);
         const int64_t pieces = ceil_div(n, sh.piece);
         const int span = EMB_THREADS / sh.G * sh.piece;

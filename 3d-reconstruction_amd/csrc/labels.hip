@@ -451,15 +451,21 @@ __global__ __launch_bounds__(LP_THREADS) void label_long_fwd_kernel(LpFwd a, int
   }
 }
 
-// joins the segments of a row
+// Joins the segments of a row: a wave, a lane to each segment.  A segment's keys come in order, so that the best of the
+// row is among the lanes' first ones: whichever lane gave it goes on to its next.
 template <typename T, bool TOP>
-__global__ __launch_bounds__(LP_THREADS) void label_join_kernel(LpFwd a, int segments, const T* __restrict__ logits,
-                                                                const LpPart* __restrict__ parts,
-                                                                const uint64_t* __restrict__ keys) {
+__global__ __launch_bounds__(64) void label_join_kernel(LpFwd a, int segments, const T* __restrict__ logits,
+                                                        const LpPart* __restrict__ parts, const uint64_t* __restrict__ keys) {
   const int64_t r = blockIdx.x;
   const T* row = logits + r * a.stride;
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x;
   static_assert(LP_SEGMENTS <= 64, "a lane takes one segment");
+  extern __shared__ uint64_t list[];  // [segments][top]
+  if constexpr (TOP) {
+    const uint64_t* mine = keys + r * segments * a.top;
+#pragma unroll 8
+    for (int i = lane; i < segments * a.top; i += 64) list[i] = mine[i];
+  }
   LpStat st{-INFINITY, 0.f, 0.f};
   if (lane < segments) {
     const LpPart p = parts[r * segments + lane];
@@ -467,30 +473,20 @@ __global__ __launch_bounds__(LP_THREADS) void label_join_kernel(LpFwd a, int seg
   }
   st = lp_wave_join(st);
   const float ls = logf(st.s);
-  if (threadIdx.x == 0) lp_write_row(a, r, st, ls, row);
+  if (lane == 0) lp_write_row(a, r, st, ls, row);
   if constexpr (TOP) {
-    __shared__ LpShared sh;
-    const int n = segments * a.top;
-    const uint64_t* mine = keys + r * n;
-    auto out = [&](int rank, uint64_t key) {
-      const uint32_t j = lp_key_index(key);
-      lp_write_top(a, r, rank, j, (float)row[j], st.m, ls);
-    };
-    if (n <= LP_LIST) {
-      for (int i = threadIdx.x; i < n; i += LP_THREADS) sh.list[i] = mine[i];
-      __syncthreads();
-      lp_rank_list(sh.list, n, a.top, out);
-    } else {
-      uint64_t below = ~0ull;
-      for (int t = 0; t < a.top; ++t) {
-        uint64_t best = 0;
-        for (int i = threadIdx.x; i < n; i += LP_THREADS) {
-          const uint64_t k = mine[i];
-          if (k < below && k > best) best = k;
-        }
-        below = lp_block_max(best, sh.best);
-        if (threadIdx.x == 0) out(t, below);
-      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    int at = 0;
+    uint64_t head = lane < segments ? list[lane * a.top] : 0ull, won = 0;
+    for (int t = 0; t < a.top; ++t) {
+      const uint64_t best = lp_wave_max(head);
+      if (lane == t) won = best;
+      if (head == best) head = ++at < a.top ? list[lane * a.top + at] : 0ull;  // (keys are distinct; zeros are none)
+    }
+    if (lane < a.top) {
+      const uint32_t j = lp_key_index(won);
+      lp_write_top(a, r, lane, j, (float)row[j], st.m, ls);
     }
   }
 }
@@ -732,7 +728,8 @@ extern "C" int gs_label_log_probs_fwd(int64_t rows, int32_t K, int32_t dtype, in
     GS_CHECK_LAUNCH();
     if (segments == 1) return GS_OK;
     if (top_k > 0)
-      hipLaunchKernelGGL((label_join_kernel<T, true>), dim3((unsigned)rows), block, 0, s, a, segments, x, parts, keys);
+      hipLaunchKernelGGL((label_join_kernel<T, true>), dim3((unsigned)rows), dim3(64), 8 * segments * top_k, s, a, segments,
+                         x, parts, keys);
     else
       hipLaunchKernelGGL((label_join_kernel<T, false>), dim3((unsigned)rows), dim3(64), 0, s, a, segments, x, parts, keys);
     GS_CHECK_LAUNCH();

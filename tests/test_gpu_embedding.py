@@ -63,6 +63,36 @@ def test_against_the_formula(gpu_device, dtype, n, V, D, kind):
     _check(f"{dtype} {n}x{V}x{D} {kind}", gpu_device, table, _ids(kind, n, V, g), 1.7, v_out)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,V,D", [(16384, 70, 20), (16385, 70, 20), (40_000, 5000, 24), (70_001, 300, 33), (300_000, 64, 16),
+                                   (300_000, 65, 16), (300_000, 3, 5), (131_072, 70_000, 8), (100_003, 1000, 704), (20_000, 7, 300),
+                                   (257, 64, 1), (5000, 1, 256), (66_000, 1 << 20, 2), (17_000, 300_000, 1)])
+@pytest.mark.parametrize("kind", ["uniform", "grouped", "skewed", "one", "outside"])
+def test_many_ids(gpu_device, dtype, n, V, D, kind):
+    """Every sort, the form for few rows, and both lengths of a piece."""
+    from gsplat.prepass import embedding_lookup
+
+    dev = gpu_device
+    g = torch.Generator().manual_seed(n + V + D)
+    ids = torch.randint(0, V, (n,), generator=g)
+    if kind == "grouped":
+        ids = ids.sort().values
+    elif kind == "skewed":
+        ids = (torch.rand(n, generator=g) ** 8 * V).long().clamp_(max=V - 1)
+    elif kind == "one":
+        ids = torch.full_like(ids, V - 1)
+    elif kind == "outside":
+        ids = torch.where(torch.rand(n, generator=g) < 0.5, torch.randint(-3, V + 4, (n,), generator=g), -1)
+    table = torch.randn(V, D, generator=g).to(dtype).to(dev).requires_grad_(True)
+    up = torch.randn(n, D, generator=g).to(dtype)
+    (v,) = torch.autograd.grad(embedding_lookup(table, ids.to(dev), 0.25), table, up.to(dev))
+    row = torch.where((ids >= 0) & (ids < V), ids, torch.full_like(ids, V))
+    ref, size = (torch.zeros(V + 1, D, dtype=torch.float64).index_add_(0, row, t)[:V] * 0.25 for t in (up.double(), up.double().abs()))
+    count = torch.bincount(row, minlength=V + 1)[:V].double()
+    assert_within(f"{dtype} {n}x{V}x{D} {kind}", v, ref, (count[:, None] + 1) * U * size + rounding(dtype, ref))
+    assert bool((v[(count == 0).to(dev)] == 0).all())
+
+
 @pytest.mark.parametrize("n", [0, 63, 64, 65, 128, 129, 255, 300, 4096, 4160])
 def test_run_lengths_around_the_pieces(gpu_device, n):
     """Runs that end at, before and behind the pieces a long run is cut into, next to short ones."""
@@ -71,6 +101,11 @@ def test_run_lengths_around_the_pieces(gpu_device, n):
     ids = torch.cat(runs)[torch.randperm(sum(len(r) for r in runs), generator=g)]
     table, v_out = torch.randn(11, 33, generator=g), torch.randn(len(ids), 33, generator=g)
     _check(f"runs {n}", gpu_device, table, ids, 1.0, v_out)
+    for short in (15, 16, 17, 31, 32, 33):  # and pieces of 16, in a table too large for the form for few rows
+        runs = [torch.full((m,), 7 * k) for k, m in enumerate((n, 1, short, 1, short + 1, 15, 16, 17, short, 47, 48, 49, 2))]
+        ids = torch.cat(runs)[torch.randperm(sum(len(r) for r in runs), generator=g)]
+        table, v_out = torch.randn(97, 9, generator=g), torch.randn(len(ids), 9, generator=g)
+        _check(f"runs {n} {short}", gpu_device, table, ids, 1.0, v_out)
 
 
 def test_strides_shapes_types_and_alignment(gpu_device):
