@@ -14,7 +14,8 @@ namespace gs {
 
 constexpr int GR_MAX_TENSORS = 128;  // 29 bytes each: the table stays within the 4 KiB of kernel arguments
 constexpr int GR_THREADS = 256;
-constexpr int GR_CHUNK_VECS = 2048;  // 16-byte vectors of one chunk (32 KiB)
+constexpr int GR_FLIGHT = 8;         // 16-byte vectors a thread has in flight
+constexpr int GR_CHUNK_VECS = GR_FLIGHT * GR_THREADS;  // vectors of one chunk (32 KiB)
 constexpr int GR_MAX_BLOCKS = 2048;  // eight workgroups on each of 256 CUs
 constexpr int GR_MAX_PARTIALS = 4096;
 
@@ -72,13 +73,21 @@ template <typename T> __device__ __forceinline__ double gr_chunk_squares(const T
   const GradSpan<T> s(src, numel);
   double acc = 0.0;
   const int64_t v0 = chunk * GR_CHUNK_VECS;
-  const int64_t v1 = v0 + GR_CHUNK_VECS < s.vecs ? v0 + GR_CHUNK_VECS : s.vecs;
-  const T* body = src + s.head;
-  for (int64_t v = v0 + threadIdx.x; v < v1; v += GR_THREADS) {
+  const T* body = src + (s.head + v0 * VE);
+  auto add = [&](const Raw<T, VE>& raw) {
     float f[VE];
-    load_vec<T, VE>(body + v * VE, f);
+    unpack<T, VE>(raw, f);
 #pragma unroll
     for (int k = 0; k < VE; ++k) acc += (double)f[k] * (double)f[k];
+  };
+  if (v0 + GR_CHUNK_VECS <= s.vecs) {  // a whole chunk: all of a thread's vectors in flight
+    Raw<T, VE> raw[GR_FLIGHT];
+#pragma unroll
+    for (int u = 0; u < GR_FLIGHT; ++u) raw[u] = load_raw<T, VE>(body + (int64_t)(u * GR_THREADS + threadIdx.x) * VE);
+#pragma unroll
+    for (int u = 0; u < GR_FLIGHT; ++u) add(raw[u]);
+  } else {
+    for (int64_t v = threadIdx.x; v < s.vecs - v0; v += GR_THREADS) add(load_raw<T, VE>(body + v * VE));
   }
   if (chunk == 0) {
     const int64_t tail0 = s.head + s.vecs * VE;
@@ -120,25 +129,34 @@ __global__ __launch_bounds__(GR_THREADS) void grad_norm_kernel(const double* __r
   if (threadIdx.x == 0) *norm = v;
 }
 
-template <typename T> __device__ __forceinline__ void gr_chunk_scale(const T* src, T* dst, int64_t numel, int64_t chunk, float c) {
+template <bool PAST, typename T>
+__device__ __forceinline__ void gr_chunk_scale(const T* src, T* dst, int64_t numel, int64_t chunk, float c) {
   constexpr int VE = GradSpan<T>::VE;
   const GradSpan<T> s(src, numel);
   const int64_t v0 = chunk * GR_CHUNK_VECS;
-  const int64_t v1 = v0 + GR_CHUNK_VECS < s.vecs ? v0 + GR_CHUNK_VECS : s.vecs;
-  const T* body = src + s.head;
-  T* out = dst + s.head;
+  const T* body = src + (s.head + v0 * VE);
+  T* out = dst + (s.head + v0 * VE);
   const bool wide = ((((uintptr_t)src) ^ ((uintptr_t)dst)) & 15u) == 0;
-  for (int64_t v = v0 + threadIdx.x; v < v1; v += GR_THREADS) {
+  auto put = [&](int64_t v, const Raw<T, VE>& raw) {
     float f[VE];
-    load_vec<T, VE>(body + v * VE, f);
+    unpack<T, VE>(raw, f);
 #pragma unroll
     for (int k = 0; k < VE; ++k) f[k] *= c;
     if (wide) {
-      store_vec<T, VE>(out + v * VE, f);
+      if constexpr (PAST) store_vec_nt<T, VE>(out + v * VE, f); else store_vec<T, VE>(out + v * VE, f);
     } else {
 #pragma unroll
       for (int k = 0; k < VE; ++k) out[v * VE + k] = (T)f[k];
     }
+  };
+  if (v0 + GR_CHUNK_VECS <= s.vecs) {
+    Raw<T, VE> raw[GR_FLIGHT];
+#pragma unroll
+    for (int u = 0; u < GR_FLIGHT; ++u) raw[u] = load_raw<T, VE>(body + (int64_t)(u * GR_THREADS + threadIdx.x) * VE);
+#pragma unroll
+    for (int u = 0; u < GR_FLIGHT; ++u) put(u * GR_THREADS + threadIdx.x, raw[u]);
+  } else {
+    for (int64_t v = threadIdx.x; v < s.vecs - v0; v += GR_THREADS) put(v, load_raw<T, VE>(body + v * VE));
   }
   if (chunk == 0) {
     const int64_t tail0 = s.head + s.vecs * VE;
@@ -147,6 +165,7 @@ template <typename T> __device__ __forceinline__ void gr_chunk_scale(const T* sr
   }
 }
 
+template <bool PAST>
 __global__ __launch_bounds__(GR_THREADS) void grad_scale_kernel(GradTable t, const double* __restrict__ partials, int n_partials,
                                                                 float max_norm, float eps, int in_place, int write_norm,
                                                                 float* __restrict__ norm) {
@@ -160,9 +179,9 @@ __global__ __launch_bounds__(GR_THREADS) void grad_scale_kernel(GradTable t, con
     const int i = gr_tensor(t, k);
     const int64_t at = k - t.first_chunk[i];
     switch (t.dtype[i]) {
-      case GS_DTYPE_F32: gr_chunk_scale((const float*)t.src[i], (float*)t.dst[i], t.numel[i], at, c); break;
-      case GS_DTYPE_BF16: gr_chunk_scale((const bf16_t*)t.src[i], (bf16_t*)t.dst[i], t.numel[i], at, c); break;
-      default: gr_chunk_scale((const f16_t*)t.src[i], (f16_t*)t.dst[i], t.numel[i], at, c); break;
+      case GS_DTYPE_F32: gr_chunk_scale<PAST>((const float*)t.src[i], (float*)t.dst[i], t.numel[i], at, c); break;
+      case GS_DTYPE_BF16: gr_chunk_scale<PAST>((const bf16_t*)t.src[i], (bf16_t*)t.dst[i], t.numel[i], at, c); break;
+      default: gr_chunk_scale<PAST>((const f16_t*)t.src[i], (f16_t*)t.dst[i], t.numel[i], at, c); break;
     }
   }
 }
@@ -231,7 +250,13 @@ static int gr_run(int32_t n, const void* const* src, void* const* dst, const int
   if (workspace_bytes < gs_grad_norm_workspace_bytes(n)) return GS_ERR_WORKSPACE;
   const int launches = n > 0 ? (int)ceil_div(n, GR_MAX_TENSORS) : 0;
   bool in_place = dst != nullptr;
-  for (int32_t t = 0; dst && t < n; ++t) in_place = in_place && (numel[t] == 0 || src[t] == dst[t]);
+  int64_t elsewhere = 0;  // bytes that are written to another place than they come from
+  for (int32_t t = 0; dst && t < n; ++t)
+    if (numel[t] > 0 && src[t] != dst[t]) {
+      in_place = false;
+      elsewhere += numel[t] * dtype_size(dtype[t]);
+    }
+  const bool past = elsewhere >= PAST_CACHES_MIN_BYTES;
   double* partials = (double*)workspace;
   int n_partials = 0;
   for (int pass = 0; pass < 2; ++pass) {
@@ -256,8 +281,9 @@ static int gr_run(int32_t n, const void* const* src, void* const* dst, const int
         hipLaunchKernelGGL(grad_squares_kernel, dim3(blocks), dim3(GR_THREADS), 0, s, tab, partials + n_partials);
         n_partials += blocks;
       } else {
-        hipLaunchKernelGGL(grad_scale_kernel, dim3(blocks), dim3(GR_THREADS), 0, s, tab, partials, n_partials, max_norm,
-                           eps, in_place ? 1 : 0, l == 0 ? 1 : 0, norm);
+        auto* kernel = past ? &grad_scale_kernel<true> : &grad_scale_kernel<false>;
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(GR_THREADS), 0, s, tab, partials, n_partials, max_norm, eps,
+                           in_place ? 1 : 0, l == 0 ? 1 : 0, norm);
       }
       GS_CHECK_LAUNCH();
     }

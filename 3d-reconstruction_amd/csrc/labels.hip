@@ -19,6 +19,7 @@ constexpr int LP_THREADS = 256;
 constexpr int LP_SMALL = 64;       // classes up to which a lane takes a whole row
 constexpr int LP_WAVE = 2048;      // classes up to which a wave holds a row in registers
 constexpr int LP_SEGMENTS = 64;    // parts a long row is cut into at most
+constexpr int LP_ADD = 16;         // values added to the statistics at a time
 constexpr int LP_LIST = 1024;      // candidates for the top alternatives that a workgroup lists
 constexpr float LP_LOG2E = 1.44269504088896340736f;
 constexpr float LP_LOW = -1.0e4f;  // stands for -inf next to an exponential that is 0 there: 0 * LP_LOW is 0
@@ -55,13 +56,11 @@ __device__ __forceinline__ LpStat lp_join(const LpStat& a, const LpStat& b) {
   return {m, ea * a.s + eb * b.s, ea * (a.w + fmaxf(da, LP_LOW) * a.s) + eb * (b.w + fmaxf(db, LP_LOW) * b.s)};
 }
 
-__device__ __forceinline__ LpStat lp_wave_join(LpStat st) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const LpStat b{__shfl_xor(st.m, o), __shfl_xor(st.s, o), __shfl_xor(st.w, o)};
-    st = lp_join(st, b);
-  }
-  return st;
+// all lanes scale to the wave's maximum once, then add up
+__device__ __forceinline__ LpStat lp_wave_join(const LpStat& st) {
+  const float m = wave_max_all(st.m), ref = m == -INFINITY ? 0.f : m;
+  const float d = st.m - ref, e = lp_exp(d);
+  return {m, wave_sum_all(e * st.s), wave_sum_all(e * (st.w + fmaxf(d, LP_LOW) * st.s))};
 }
 
 // a total order of logits: larger first, NaN above all, equal values (and the two zeros) by the lower index
@@ -73,26 +72,20 @@ __device__ __forceinline__ uint32_t lp_order(float x) {
 __device__ __forceinline__ float lp_value(uint32_t order) {  // of an order that is not NaN's
   return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
 }
+// the largest value that no order from `order` on is below; -inf for those below that of -inf
+__device__ __forceinline__ float lp_least(uint32_t order) { return lp_value(order > 0x007fffffu ? order : 0x007fffffu); }
 __device__ __forceinline__ uint64_t lp_key(float x, uint32_t j) { return ((uint64_t)lp_order(x) << 32) | (uint32_t)~j; }
 __device__ __forceinline__ uint32_t lp_key_index(uint64_t key) { return ~(uint32_t)key; }
 
-__device__ __forceinline__ uint64_t lp_wave_max(uint64_t v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const uint64_t w = __shfl_xor((unsigned long long)v, o);
-    v = w > v ? w : v;
-  }
-  return v;
-}
-
-// the k-th largest of the lanes' values, bit by bit
+// A value that at least k lanes reach and that the k-th largest of them is not far above: its upper half, bit by bit, and
+// no further once no other lane reaches it (what is listed from it on is ranked anyway).
 __device__ __forceinline__ uint32_t lp_wave_kth(uint32_t v, int k) {
   uint32_t found = 0;
-#pragma unroll
-  for (int b = 31; b >= 0; --b) {
-    const uint32_t want = (found >> b) | 1u;
-    const int c = __popcll(__ballot((v >> b) == want));
-    if (c >= k) found |= 1u << b; else k -= c;
+  for (int b = 31; b >= 16; --b) {
+    const uint32_t want = found | (1u << b);
+    const int c = __popcll(__ballot(v >= want));
+    if (c >= k) found = want;
+    if (c == k) break;
   }
   return found;
 }
@@ -226,10 +219,19 @@ __global__ __launch_bounds__(LP_THREADS) void label_wave_fwd_kernel(LpFwd a, con
       if (u * 64 + lane < sp.vecs) sp.load(u * 64 + lane, *reinterpret_cast<float(*)[VE]>(&x[u * VE]));
     const int ex = sp.extra(lane);
     if (ex >= 0) x[NX - 1] = (float)sp.x[ex];
-    LpStat st{-INFINITY, 0.f, 0.f};
-    lp_add<NX>(st, x);
-    const float lane_max = st.m;
-    st = lp_wave_join(st);
+    float lane_max = x[0];
+#pragma unroll
+    for (int i = 1; i < NX; ++i) lane_max = fmaxf(lane_max, x[i]);
+    LpStat st{wave_max_all(lane_max), 0.f, 0.f};
+    const float ref = st.m == -INFINITY ? 0.f : st.m;
+#pragma unroll
+    for (int i = 0; i < NX; ++i) {
+      const float d = x[i] - ref, e = lp_exp(d);
+      st.s += e;
+      st.w += e * fmaxf(d, LP_LOW);
+    }
+    st.s = wave_sum_all(st.s);
+    st.w = wave_sum_all(st.w);
     const float ls = logf(st.s);
     if (lane == 0) lp_write_row(a, r, st, ls, sp.x);
     if (a.top == 0) continue;
@@ -242,14 +244,14 @@ __global__ __launch_bounds__(LP_THREADS) void label_wave_fwd_kernel(LpFwd a, con
     // The k-th largest of the lanes' maxima is no larger than the k-th largest value: what is not below it is listed.
     int listed = 65;
     if (st.s == st.s) {  // (NaN is above all, and no lane's maximum shows it: such rows go the long way)
-      const float least = lp_value(lp_wave_kth(lp_order(lane_max), a.top));
+      const float least = lp_least(lp_wave_kth(lp_order(lane_max), a.top));
       listed = 0;
 #pragma unroll
       for (int i = 0; i < NX; ++i) {
-        const int j = index(i);
-        const bool in = j >= 0 && x[i] >= least;
-        const unsigned long long b = __ballot(in);
-        if (b) {
+        if (__ballot(x[i] >= least)) {
+          const int j = index(i);
+          const bool in = j >= 0 && x[i] >= least;
+          const unsigned long long b = __ballot(in);
           const int at = listed + __popcll(b & ((1ull << lane) - 1ull));
           if (in && at < 64) list[at] = lp_key(x[i], (uint32_t)j);
           listed += __popcll(b);
@@ -278,7 +280,7 @@ __global__ __launch_bounds__(LP_THREADS) void label_wave_fwd_kernel(LpFwd a, con
           const uint64_t k = j >= 0 ? lp_key(x[i], (uint32_t)j) : 0ull;
           if (k < below && k > best) best = k;
         }
-        best = lp_wave_max(best);
+        best = wave_max_all(best);
         below = best;
         const uint32_t j = lp_key_index(best);
         if (lane == 0) lp_write_top(a, r, t, j, (float)sp.x[j], st.m, ls);
@@ -302,10 +304,16 @@ template <typename T> __device__ __forceinline__ LpStat lp_strip(const LpSpan<T>
   LpStat st{-INFINITY, 0.f, 0.f};
   int v = threadIdx.x;
   for (; v + 3 * LP_THREADS < sp.vecs; v += 4 * LP_THREADS) {
-    float f[4 * VE];
+    Raw<T, VE> raw[4];  // (as loaded: a third of the registers, and all workgroups of a CU at once)
 #pragma unroll
-    for (int u = 0; u < 4; ++u) sp.load(v + u * LP_THREADS, *reinterpret_cast<float(*)[VE]>(&f[u * VE]));
-    lp_add<4 * VE>(st, f);
+    for (int u = 0; u < 4; ++u) raw[u] = load_raw<T, VE>(sp.x + sp.at(v + u * LP_THREADS));
+#pragma unroll
+    for (int u = 0; u < 4; u += LP_ADD / VE) {
+      float f[LP_ADD];
+#pragma unroll
+      for (int k = 0; k < LP_ADD / VE; ++k) unpack<T, VE>(raw[u + k], f + k * VE);
+      lp_add<LP_ADD>(st, f);
+    }
   }
   for (; v < sp.vecs; v += LP_THREADS) {
     float f[VE];
@@ -353,7 +361,7 @@ template <typename F> __device__ __forceinline__ void lp_rank_list(const uint64_
 
 // Largest of the workgroup's values, for all threads; two barriers.
 __device__ __forceinline__ uint64_t lp_block_max(uint64_t v, uint64_t* lds) {
-  v = lp_wave_max(v);
+  v = wave_max_all(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
   __syncthreads();
@@ -376,7 +384,7 @@ __device__ __forceinline__ void lp_block_top(const LpSpan<T>& sp, uint32_t j0, i
     uint32_t order = sh.least[0];
 #pragma unroll
     for (int w = 1; w < LP_THREADS / 64; ++w) order = sh.least[w] > order ? sh.least[w] : order;
-    const float least = lp_value(order);
+    const float least = lp_least(order);
     if (strip.m >= least)
       lp_walk(sp, [&](float x, int j) {
         if (x >= least) {
@@ -480,7 +488,7 @@ __global__ __launch_bounds__(64) void label_join_kernel(LpFwd a, int segments, c
     int at = 0;
     uint64_t head = lane < segments ? list[lane * a.top] : 0ull, won = 0;
     for (int t = 0; t < a.top; ++t) {
-      const uint64_t best = lp_wave_max(head);
+      const uint64_t best = wave_max_all(head);
       if (lane == t) won = best;
       if (head == best) head = ++at < a.top ? list[lane * a.top + at] : 0ull;  // (keys are distinct; zeros are none)
     }
@@ -569,7 +577,7 @@ __global__ __launch_bounds__(64) void label_small_bwd_kernel(LpBwd a, uint32_t m
 
 // `lanes` threads (a wave, or a workgroup) over a part of a row; the gradient's row is as far apart from a 16-byte boundary
 // as the logits' (`wide`), or is written value by value
-template <typename T, int LANES>
+template <typename T, int LANES, bool PAST>
 __device__ __forceinline__ void lp_grad_span(const LpSpan<T>& sp, const LpRow& w, int j0, int t, T* __restrict__ out) {
   constexpr int VE = LpSpan<T>::VE;
   const bool wide = (((uintptr_t)sp.x ^ (uintptr_t)out) & 15u) == 0;
@@ -585,7 +593,7 @@ __device__ __forceinline__ void lp_grad_span(const LpSpan<T>& sp, const LpRow& w
       for (int k = 0; k < VE; ++k) f[k] += y == j + k ? w.g : 0.f;
     }
     if (wide) {
-      store_vec<T, VE>(out + j, f);
+      if constexpr (PAST) store_vec_nt<T, VE>(out + j, f); else store_vec<T, VE>(out + j, f);
     } else {
 #pragma unroll
       for (int k = 0; k < VE; ++k) out[j + k] = (T)f[k];
@@ -595,7 +603,7 @@ __device__ __forceinline__ void lp_grad_span(const LpSpan<T>& sp, const LpRow& w
   if (ex >= 0) out[ex] = (T)((w.none ? 0.f : lp_grad(w, (float)sp.x[ex])) + (w.y >= 0 && ex == y ? w.g : 0.f));
 }
 
-template <typename T>
+template <typename T, bool PAST>
 __global__ __launch_bounds__(LP_THREADS) void label_wave_bwd_kernel(LpBwd a, const T* __restrict__ logits, T* __restrict__ v) {
   const int lane = threadIdx.x & 63;
   const int64_t waves = (int64_t)gridDim.x * (LP_THREADS / 64);
@@ -603,7 +611,7 @@ __global__ __launch_bounds__(LP_THREADS) void label_wave_bwd_kernel(LpBwd a, con
     const LpSpan<T> sp(logits + r * a.stride, a.K);
     const LpRow w = lp_row(a, r);
     T* out = v + r * a.K;
-    lp_grad_span<T, 64>(sp, w, 0, lane, out);
+    lp_grad_span<T, 64, PAST>(sp, w, 0, lane, out);
     if (a.g_top && !w.none) {
       __builtin_amdgcn_s_waitcnt(0);  // the row's stores are out before some of its values are stored again
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
@@ -615,7 +623,7 @@ __global__ __launch_bounds__(LP_THREADS) void label_wave_bwd_kernel(LpBwd a, con
   }
 }
 
-template <typename T>
+template <typename T, bool PAST>
 __global__ __launch_bounds__(LP_THREADS) void label_long_bwd_kernel(LpBwd a, int segments, int seg_len,
                                                                     const T* __restrict__ logits, T* __restrict__ v) {
   const int64_t items = a.rows * segments;
@@ -625,7 +633,7 @@ __global__ __launch_bounds__(LP_THREADS) void label_long_bwd_kernel(LpBwd a, int
     const LpSpan<T> sp(logits + r * a.stride + j0, a.K - j0 < seg_len ? a.K - j0 : seg_len);
     const LpRow w = lp_row(a, r);
     T* out = v + r * a.K + j0;
-    lp_grad_span<T, LP_THREADS>(sp, w, j0, threadIdx.x, out);
+    lp_grad_span<T, LP_THREADS, PAST>(sp, w, j0, threadIdx.x, out);
     if (a.g_top && !w.none) {
       __builtin_amdgcn_s_waitcnt(0);
       __syncthreads();
@@ -747,6 +755,7 @@ extern "C" int gs_label_log_probs_bwd(int64_t rows, int32_t K, int32_t dtype, in
   if (!stats || !entropy || !v_logits || (g_top_log_probs && (top_k < 1 || !top_labels))) return GS_ERR_INVALID_ARG;
   if ((uintptr_t)v_logits & (uintptr_t)(dtype_size(dtype) - 1)) return GS_ERR_INVALID_ARG;
   const LpBwd a{rows, row_stride, K, top_k, label_bytes, labels, stats, entropy, top_labels, g_log_prob, g_entropy, g_top_log_probs};
+  const bool past = rows * K * dtype_size(dtype) >= PAST_CACHES_MIN_BYTES;
   hipStream_t s = (hipStream_t)stream;
   return with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
@@ -755,13 +764,19 @@ extern "C" int gs_label_log_probs_bwd(int64_t rows, int32_t K, int32_t dtype, in
       hipLaunchKernelGGL(label_small_bwd_kernel<T>, dim3(lp_grid(rows, 64)), dim3(64), 64 * (K | 1) * sizeof(float), s, a,
                          lp_magic(K), x, (T*)v_logits);
     } else if (K <= LP_WAVE) {
-      hipLaunchKernelGGL(label_wave_bwd_kernel<T>, dim3(lp_grid(rows, LP_THREADS / 64)), dim3(LP_THREADS), 0, s, a, x,
-                         (T*)v_logits);
+      const dim3 grid(lp_grid(rows, LP_THREADS / 64)), block(LP_THREADS);
+      if (past)
+        hipLaunchKernelGGL((label_wave_bwd_kernel<T, true>), grid, block, 0, s, a, x, (T*)v_logits);
+      else
+        hipLaunchKernelGGL((label_wave_bwd_kernel<T, false>), grid, block, 0, s, a, x, (T*)v_logits);
     } else {
       int32_t seg_len;
       const int segments = lp_segments(rows, K, &seg_len);
-      hipLaunchKernelGGL(label_long_bwd_kernel<T>, dim3(lp_grid(rows * segments, 1)), dim3(LP_THREADS), 0, s, a, segments,
-                         seg_len, x, (T*)v_logits);
+      const dim3 grid(lp_grid(rows * segments, 1)), block(LP_THREADS);
+      if (past)
+        hipLaunchKernelGGL((label_long_bwd_kernel<T, true>), grid, block, 0, s, a, segments, seg_len, x, (T*)v_logits);
+      else
+        hipLaunchKernelGGL((label_long_bwd_kernel<T, false>), grid, block, 0, s, a, segments, seg_len, x, (T*)v_logits);
     }
     GS_CHECK_LAUNCH();
     return GS_OK;
