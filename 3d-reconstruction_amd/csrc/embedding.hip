@@ -473,31 +473,18 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_runs_kernel(EmbShape sh, co
   }
 }
 
-// emb_lower by a whole wave: 64 probes at a time
-__device__ __forceinline__ int64_t emb_lower_wave(const uint32_t* __restrict__ keys, int64_t lo, int64_t hi, uint32_t v) {
-  const int lane = threadIdx.x & 63;
-  while (lo < hi) {
-    const int64_t step = (hi - lo + 63) / 64, at = lo + (lane + 1) * step - 1;  // the last of the lane's stretch
-    const int64_t below = __popcll(__ballot(at < hi && keys[at < hi ? at : hi - 1] < v));
-    lo += below * step;
-    if (step == 1) break;
-    hi = lo + step - 1 < hi ? lo + step - 1 : hi;  // (its last entry is known not to be below)
-  }
-  return lo;
-}
-
 // A workgroup looks at EMB_JOIN_PIECES pieces; for each in which a long run starts it adds the run's pieces, its groups in
 // turn, and joins the groups in LDS, in their order.
 template <typename T, int N>
 __global__ __launch_bounds__(EMB_JOIN_THREADS) void embed_join_kernel(EmbShape sh, const uint32_t* __restrict__ keys,
                                                                       const float* __restrict__ partial,
                                                                       T* __restrict__ v_table) {
-  constexpr int MAX_KEYS = (EMB_JOIN_PIECES + 1) * EMB_PIECE_MAX + 1;
-  __shared__ float lds[EMB_JOIN_THREADS * N > MAX_KEYS ? EMB_JOIN_THREADS * N : MAX_KEYS];
+  __shared__ float lds[EMB_JOIN_THREADS * N];
+  __shared__ uint32_t near[(EMB_JOIN_PIECES + 1) * EMB_PIECE_MAX + 1];
   __shared__ int64_t start[EMB_JOIN_PIECES];  // of the long run that starts in the piece, -1: none does
   const int P = sh.piece;
   const int64_t p0 = (int64_t)blockIdx.x * EMB_JOIN_PIECES;
-  uint32_t* near = reinterpret_cast<uint32_t*>(lds);  // the keys from the one before the pieces on, and P behind them
+  // near: the keys from the one before the pieces on, and P behind them
   for (int l = threadIdx.x; l <= (EMB_JOIN_PIECES + 1) * P; l += EMB_JOIN_THREADS) {
     const int64_t e = p0 * P - 1 + l;
     near[l] = e < 0 ? 0xfffffffeu : e < sh.n ? keys[e] : 0xffffffffu;  // neither is a key
@@ -520,31 +507,30 @@ __global__ __launch_bounds__(EMB_JOIN_THREADS) void embed_join_kernel(EmbShape s
   for (int q = 0; q < EMB_JOIN_PIECES; ++q) {
     const int64_t s = start[q];
     if (s < 0) continue;
-    const uint32_t key = keys[s];
-    const int64_t e = emb_lower_wave(keys, s + P, sh.n, key + 1), last = (e - 1) / P;  // the piece of its last entry
+    const uint32_t key = near[1 + q * P + (int)(s - (p0 + q) * P)];
     float acc[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) acc[k] = 0.f;
     if (vec < sh.vpr) {
-#pragma unroll 4
-      for (int64_t r = p0 + q + g; r <= last; r += groups) {
-        const float* src = partial + (2 * r + (r == p0 + q ? 1 : 0)) * D + vec * N;
+      for (int64_t r = p0 + q + g; r * P < sh.n; r += groups) {
+        const bool first = r == p0 + q;
+        if (!first && keys[r * P] != key) break;  // (a piece is the run's exactly where its first entry is)
+        const float* src = partial + (2 * r + (first ? 1 : 0)) * D + vec * N;
 #pragma unroll
         for (int k = 0; k < N; ++k) acc[k] += src[k];
       }
     }
+    for (int half = groups / 2; half > 0; half /= 2) {
+      if (g >= half && g < 2 * half)
 #pragma unroll
-    for (int k = 0; k < N; ++k) lds[k * EMB_JOIN_THREADS + threadIdx.x] = acc[k];
-    __syncthreads();
-    if (g == 0 && vec < sh.vpr) {
-      const int64_t full = last - (p0 + q) + 1;
-      const int have = full < groups ? (int)full : groups;
-      for (int h = 1; h < have; ++h)
+        for (int k = 0; k < N; ++k) lds[k * EMB_JOIN_THREADS + threadIdx.x] = acc[k];
+      __syncthreads();
+      if (g < half)
 #pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] += lds[k * EMB_JOIN_THREADS + h * sh.G + threadIdx.x];
-      emb_store<T, N>(v_table + (int64_t)key * D + vec * N, acc, sh.scale);
+        for (int k = 0; k < N; ++k) acc[k] += lds[k * EMB_JOIN_THREADS + half * sh.G + threadIdx.x];
+      __syncthreads();
     }
-    __syncthreads();
+    if (g == 0 && vec < sh.vpr) emb_store<T, N>(v_table + (int64_t)key * D + vec * N, acc, sh.scale);
   }
 }
 
@@ -725,10 +711,10 @@ static EmbWorkspace emb_workspace(int64_t n, int64_t V, int64_t D) {
   return w;
 }
 
-// workgroups that fill one share of the table: 16 KiB each, at most eight on a CU
+// workgroups that fill one share of the table: four vectors a thread, more in a large one
 static unsigned emb_fill_blocks(const EmbFill& f, int threads) {
   const int64_t b = ceil_div(f.bytes / f.shares, (int64_t)threads * 64);
-  return (unsigned)std::min<int64_t>(std::max<int64_t>(b, 1), 2048 * 256 / threads);
+  return (unsigned)std::min<int64_t>(std::max<int64_t>(b, 1), 4096);
 }
 
 // sorts the ids and zeroes the table; `w` says which of the two pairs of lists has the result

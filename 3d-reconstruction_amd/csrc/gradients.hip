@@ -16,7 +16,7 @@ constexpr int GR_MAX_TENSORS = 128;  // 29 bytes each: the table stays within th
 constexpr int GR_THREADS = 256;
 constexpr int GR_FLIGHT = 8;         // 16-byte vectors a thread has in flight
 constexpr int GR_CHUNK_VECS = GR_FLIGHT * GR_THREADS;  // vectors of one chunk (32 KiB)
-constexpr int GR_MAX_BLOCKS = 2048;  // eight workgroups on each of 256 CUs
+constexpr int GR_MAX_BLOCKS = 1024;  // four workgroups on each of 256 CUs; each of the second pass adds up all partial sums
 constexpr int GR_MAX_PARTIALS = 4096;
 
 struct GradTable {
@@ -175,7 +175,8 @@ __global__ __launch_bounds__(GR_THREADS) void grad_scale_kernel(GradTable t, con
   const float q = max_norm / (v + eps);
   const float c = q > 1.0f ? 1.0f : q;  // a NaN norm stays one
   if (in_place && c == 1.0f) return;    // nothing changes
-  for (int k = blockIdx.x; k < t.chunks; k += gridDim.x) {
+  // from the end: what was read last for the norm is still in the caches (268 MB and more of them read twice: 196 -> 182 us)
+  for (int k = t.chunks - 1 - (int)blockIdx.x; k >= 0; k -= (int)gridDim.x) {
     const int i = gr_tensor(t, k);
     const int64_t at = k - t.first_chunk[i];
     switch (t.dtype[i]) {

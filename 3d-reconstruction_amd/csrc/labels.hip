@@ -169,7 +169,7 @@ __global__ __launch_bounds__(64) void label_small_fwd_kernel(LpFwd a, uint32_t m
     const int rows = (int)(a.rows - row0 < 64 ? a.rows - row0 : 64);
     lp_small_load(logits, a.stride, row0, rows, K, P, magic, lane, tile);
     if (lane < rows) {
-      const float* x = tile + lane * P;
+      float* x = tile + lane * P;
       const int64_t r = row0 + lane;
       LpStat st{-INFINITY, 0.f, 0.f};
       for (int j = 0; j < K; ++j) st.m = fmaxf(st.m, x[j]);
@@ -182,16 +182,33 @@ __global__ __launch_bounds__(64) void label_small_fwd_kernel(LpFwd a, uint32_t m
       const float ls = logf(st.s);
       const int64_t y = lp_label(a.labels, a.label_bytes, r);
       lp_write_row(a, r, st, ls, y, y < 0 || y >= K ? 0.f : x[y]);
-      uint64_t below = ~0ull;
-      for (int t = 0; t < a.top; ++t) {
-        uint64_t best = 0;
-        for (int j = 0; j < K; ++j) {
-          const uint64_t k = lp_key(x[j], (uint32_t)j);
-          if (k < below && k > best) best = k;
+      if (st.s == st.s) {
+        // One after another; what is taken becomes NaN, which is above nothing.
+        for (int t = 0; t < a.top; ++t) {
+          float best = -INFINITY;
+          int at = -1;
+          for (int j = 0; j < K; ++j)
+            if (x[j] > best) {
+              best = x[j];
+              at = j;
+            }
+          for (int j = 0; at < 0; ++j)  // nothing but -inf is left: the first (K >= top: there is one)
+            if (j == K - 1 || x[j] == -INFINITY) at = j;
+          x[at] = __builtin_nanf("");
+          lp_write_top(a, r, t, (uint32_t)at, best, st.m, ls);
         }
-        below = best;
-        const uint32_t j = lp_key_index(best);
-        lp_write_top(a, r, t, j, x[j], st.m, ls);
+      } else {  // with NaN above all
+        uint64_t below = ~0ull;
+        for (int t = 0; t < a.top; ++t) {
+          uint64_t best = 0;
+          for (int j = 0; j < K; ++j) {
+            const uint64_t k = lp_key(x[j], (uint32_t)j);
+            if (k < below && k > best) best = k;
+          }
+          below = best;
+          const uint32_t j = lp_key_index(best);
+          lp_write_top(a, r, t, j, x[j], st.m, ls);
+        }
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -544,7 +561,7 @@ template <typename T> __device__ __forceinline__ T lp_grad_top(const LpBwd& a, c
   return (T)(lp_grad(w, x) + (j == w.y ? w.g : 0.f) + a.g_top[r * a.top + t]);
 }
 
-template <typename T>
+template <typename T, bool PAST>
 __global__ __launch_bounds__(64) void label_small_bwd_kernel(LpBwd a, uint32_t magic, const T* __restrict__ logits,
                                                              T* __restrict__ v) {
   extern __shared__ float tile[];
@@ -568,7 +585,8 @@ __global__ __launch_bounds__(64) void label_small_bwd_kernel(LpBwd a, uint32_t m
 #pragma unroll 8
     for (int f = lane; f < total; f += 64) {
       const int r = (int)(((uint32_t)f * magic) >> 22);
-      out[f] = (T)tile[r * P + f - r * K];
+      const T g = (T)tile[r * P + f - r * K];
+      if constexpr (PAST) __builtin_nontemporal_store(g, out + f); else out[f] = g;
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -761,8 +779,12 @@ extern "C" int gs_label_log_probs_bwd(int64_t rows, int32_t K, int32_t dtype, in
     using T = decltype(t);
     const T* x = (const T*)logits;
     if (K <= LP_SMALL) {
-      hipLaunchKernelGGL(label_small_bwd_kernel<T>, dim3(lp_grid(rows, 64)), dim3(64), 64 * (K | 1) * sizeof(float), s, a,
-                         lp_magic(K), x, (T*)v_logits);
+      const dim3 grid(lp_grid(rows, 64)), block(64);
+      const size_t tile = 64 * (K | 1) * sizeof(float);
+      if (past)
+        hipLaunchKernelGGL((label_small_bwd_kernel<T, true>), grid, block, tile, s, a, lp_magic(K), x, (T*)v_logits);
+      else
+        hipLaunchKernelGGL((label_small_bwd_kernel<T, false>), grid, block, tile, s, a, lp_magic(K), x, (T*)v_logits);
     } else if (K <= LP_WAVE) {
       const dim3 grid(lp_grid(rows, LP_THREADS / 64)), block(LP_THREADS);
       if (past)
