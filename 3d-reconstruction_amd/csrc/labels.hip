@@ -19,6 +19,9 @@ constexpr int LP_THREADS = 256;
 constexpr int LP_SMALL = 64;       // classes up to which a lane takes a whole row
 constexpr int LP_WAVE = 2048;      // classes up to which a wave holds a row in registers
 constexpr int LP_SEGMENTS = 64;    // parts a long row is cut into at most
+constexpr int LP_BLOCKS_FWD = 1024;  // workgroups that the rows are cut into segments for: four a CU, as segments cost a join
+constexpr int LP_BLOCKS_BWD = 8192;
+constexpr int LP_FLIGHT = 4;       // vectors a thread of the gradient has in flight
 constexpr int LP_ADD = 16;         // values added to the statistics at a time
 constexpr int LP_LIST = 1024;      // candidates for the top alternatives that a workgroup lists
 constexpr float LP_LOG2E = 1.44269504088896340736f;
@@ -600,9 +603,9 @@ __device__ __forceinline__ void lp_grad_span(const LpSpan<T>& sp, const LpRow& w
   constexpr int VE = LpSpan<T>::VE;
   const bool wide = (((uintptr_t)sp.x ^ (uintptr_t)out) & 15u) == 0;
   const int y = (int)(w.y - j0);  // the label's place in this part, if it is in it
-  for (int v = t; v < sp.vecs; v += LANES) {
+  auto put = [&](int v, const Raw<T, VE>& raw) {
     float f[VE];
-    sp.load(v, f);
+    unpack<T, VE>(raw, f);
 #pragma unroll
     for (int k = 0; k < VE; ++k) f[k] = w.none ? 0.f : lp_grad(w, f[k]);
     const int j = sp.at(v);
@@ -616,7 +619,16 @@ __device__ __forceinline__ void lp_grad_span(const LpSpan<T>& sp, const LpRow& w
 #pragma unroll
       for (int k = 0; k < VE; ++k) out[j + k] = (T)f[k];
     }
+  };
+  int v = t;
+  for (; v + (LP_FLIGHT - 1) * LANES < sp.vecs; v += LP_FLIGHT * LANES) {
+    Raw<T, VE> raw[LP_FLIGHT];
+#pragma unroll
+    for (int u = 0; u < LP_FLIGHT; ++u) raw[u] = load_raw<T, VE>(sp.x + sp.at(v + u * LANES));
+#pragma unroll
+    for (int u = 0; u < LP_FLIGHT; ++u) put(v + u * LANES, raw[u]);
   }
+  for (; v < sp.vecs; v += LANES) put(v, load_raw<T, VE>(sp.x + sp.at(v)));
   const int ex = sp.extra(t);
   if (ex >= 0) out[ex] = (T)((w.none ? 0.f : lp_grad(w, (float)sp.x[ex])) + (w.y >= 0 && ex == y ? w.g : 0.f));
 }
@@ -681,9 +693,9 @@ static unsigned lp_grid(int64_t items, int per_block) {
   return (unsigned)(b < (1 << 20) ? b : (1 << 20));  // (the kernels go on to further items)
 }
 
-// Segments of a long row: about a thousand workgroups in all (four a CU), none shorter than a vector for each thread.
-static int lp_segments(int64_t rows, int32_t K, int32_t* seg_len) {
-  int64_t n = rows >= 1024 ? 1 : ceil_div(1024, rows);
+// Segments of a long row: about `blocks` workgroups in all, none shorter than a vector for each thread.
+static int lp_segments(int64_t rows, int32_t K, int64_t blocks, int32_t* seg_len) {
+  int64_t n = rows >= blocks ? 1 : ceil_div(blocks, rows);
   n = std::min<int64_t>(n, std::min<int64_t>(LP_SEGMENTS, ceil_div(K, 2048)));
   *seg_len = (int32_t)(ceil_div(ceil_div(K, n), 64) * 64);
   return (int)ceil_div(K, *seg_len);
@@ -705,7 +717,7 @@ static int64_t lp_parts_bytes(int64_t items) { return ceil_div(items * (int64_t)
 extern "C" int64_t gs_label_log_probs_workspace_bytes(int64_t rows, int32_t K, int32_t top_k) {
   if (rows <= 0 || K <= gs::LP_WAVE || top_k < 0) return 0;
   int32_t seg_len;
-  const int64_t segments = gs::lp_segments(rows, K, &seg_len);
+  const int64_t segments = gs::lp_segments(rows, K, gs::LP_BLOCKS_FWD, &seg_len);
   return segments == 1 ? 0 : gs::lp_parts_bytes(rows * segments) + 8 * rows * segments * top_k;
 }
 
@@ -743,7 +755,7 @@ extern "C" int gs_label_log_probs_fwd(int64_t rows, int32_t K, int32_t dtype, in
         return GS_ERR_INVALID_ARG;
       });
     int32_t seg_len;
-    const int segments = lp_segments(rows, K, &seg_len);
+    const int segments = lp_segments(rows, K, LP_BLOCKS_FWD, &seg_len);
     LpPart* parts = (LpPart*)workspace;
     uint64_t* keys = (uint64_t*)((char*)workspace + lp_parts_bytes(rows * segments));
     const dim3 grid(lp_grid(rows * segments, 1)), block(LP_THREADS);
@@ -793,7 +805,7 @@ extern "C" int gs_label_log_probs_bwd(int64_t rows, int32_t K, int32_t dtype, in
         hipLaunchKernelGGL((label_wave_bwd_kernel<T, false>), grid, block, 0, s, a, x, (T*)v_logits);
     } else {
       int32_t seg_len;
-      const int segments = lp_segments(rows, K, &seg_len);
+      const int segments = lp_segments(rows, K, LP_BLOCKS_BWD, &seg_len);
       const dim3 grid(lp_grid(rows * segments, 1)), block(LP_THREADS);
       if (past)
         hipLaunchKernelGGL((label_long_bwd_kernel<T, true>), grid, block, 0, s, a, segments, seg_len, x, (T*)v_logits);
