@@ -93,14 +93,6 @@ struct EmbShape {
   float scale;
 };
 
-template <typename T, int N>
-__device__ __forceinline__ void emb_add(float (&acc)[N], const T* __restrict__ v_out, int64_t gs, int64_t pos, int64_t col) {
-  float x[N];
-  load_vec<T, N>(v_out + pos * gs + col, x);
-#pragma unroll
-  for (int k = 0; k < N; ++k) acc[k] += x[k];
-}
-
 // The sorted sums go past the caches: the rows of v_out that are still to be read stay there instead.  200003 ids on
 // 32000 x 512 bf16, lookup and gradient: 176 -> 146 us, 187 -> 158 us with a pass over the gradient behind it.
 template <typename T, int N, bool NT = true>
@@ -648,8 +640,17 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_direct_kernel(EmbShape sh, 
     float acc[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) acc[k] = 0.f;
-    for (int h = 0; h < hits; ++h)
-      if (hit_row[h] == r) emb_add<T, N>(acc, v_out, sh.gs, (int64_t)hit_pos[h], vec * N);
+    for (int h = 0; h < hits; h += 8) {  // (all of the ids may be one row's)
+      float x[8][N];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (h + u < hits && hit_row[h + u] == r) load_vec<T, N>(v_out + (int64_t)hit_pos[h + u] * sh.gs + vec * N, x[u]);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (h + u < hits && hit_row[h + u] == r)
+#pragma unroll
+          for (int k = 0; k < N; ++k) acc[k] += x[u][k];
+    }
     emb_store<T, N, false>(v_table + (v0 + r) * sh.vpr * N + vec * N, acc, sh.scale);
   }
 }

@@ -3,9 +3,13 @@
 // that runs in the engine's thread without the interpreter); the arithmetic is libgsplat_mi355x's, whose entry points are
 // looked up in the library that the package has loaded.  Measured on a lookup of one id with its gradient: 101 us with a
 // Python autograd node over ctypes, 41 us of it the empty node alone; see also the table of the operators' times.
+#include <c10/core/impl/VirtualGuardImpl.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/extension.h>
 
 #include "../../include/gsplat_mi355x.h"
@@ -93,6 +97,28 @@ Tensor once(const Tensor& v, const char* what) {
   return (*fail)({v.detach().requires_grad_(true)})[0];
 }
 
+// Called by a backward before it launches anything.  While a graph captures the backward, a leaf whose gradient would be
+// accumulated on another stream (an eager graph of that leaf, still alive, has made the node that does it) would pull that
+// stream into the capture, which ends the process: an error instead.
+void check_capture(const Tensor& grad) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  const auto* tasks = torch::autograd::get_current_graph_task_exec_info();
+  const c10::Stream here = c10::impl::VirtualGuardImpl(grad.device().type()).getStream(grad.device());
+  for (const auto& edge : node->next_edges()) {
+    auto* leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get());
+    if (!leaf) continue;
+    if (tasks && !tasks->empty()) {  // torch.autograd.grad: nothing is accumulated
+      const auto it = tasks->find(leaf);
+      if (it == tasks->end() || !it->second.needed_) continue;
+    }
+    const auto there = leaf->stream();
+    TORCH_CHECK(!there || *there == here, "gsplat (MI355X build): this backward is being captured while an eager graph of the "
+                "same leaf, made on another stream, is alive: delete its outputs before the capture");
+  }
+}
+
 // ---------------------------------------------------------------------------------------------------------- embedding
 struct EmbeddingLookup : torch::autograd::Function<EmbeddingLookup> {
   static Tensor forward(AutogradContext* ctx, const Tensor& table, const Tensor& ids, double scale) {
@@ -111,6 +137,7 @@ struct EmbeddingLookup : torch::autograd::Function<EmbeddingLookup> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_capture(grads[0]);
     const Tensor flat = ctx->get_saved_variables()[0];
     const double scale = ctx->saved_data["scale"].toDouble();
     const int64_t V = ctx->saved_data["rows"].toInt(), n = flat.numel(), D = grads[0].size(-1);
@@ -158,6 +185,7 @@ struct LabelLogProbs : torch::autograd::Function<LabelLogProbs> {
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
+    check_capture(saved[0]);
     const Tensor &x = saved[0], &y = saved[1], &stats = saved[2], &entropy = saved[3], &top_idx = saved[4];
     const int64_t rows = x.size(0), K = x.size(1), top_k = top_idx.size(1);
     Tensor g[3];

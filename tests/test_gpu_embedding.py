@@ -255,3 +255,32 @@ def test_refusals_on_the_device(gpu_device):
     (v,) = torch.autograd.grad(embedding_lookup(leaf, ids).square().sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError, match="cannot be differentiated twice"):
         v.sum().backward()
+
+
+@pytest.mark.parametrize("n", [100, 256])
+def test_few_ids_of_one_row(gpu_device, n):
+    g = torch.Generator().manual_seed(n)
+    table, v_out = torch.randn(500, 24, generator=g), torch.randn(n, 24, generator=g)
+    _check(f"one row {n}", gpu_device, table, torch.full((n,), 77), 1.0, v_out)
+
+
+def test_captured_backward_next_to_an_eager_graph_is_refused(gpu_device):
+    """An eager graph of the same leaf, made on another stream and still alive, would pull that stream into the capture."""
+    from gsplat.losses import label_log_probs
+    from gsplat.prepass import embedding_lookup
+
+    dev = gpu_device
+    table = torch.randn(20, 8, device=dev).requires_grad_(True)
+    ids, labels = torch.arange(20, device=dev), torch.arange(20, device=dev) % 8
+    for make in (lambda: embedding_lookup(table, ids).sum(), lambda: label_log_probs(table, labels).log_prob.sum()):
+        make().backward()  # (warm)
+        table.grad = None
+        eager = make()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="eager graph of the same leaf"):
+            with torch.cuda.graph(graph):
+                make().backward()
+        eager.backward()
+        assert bool(torch.isfinite(table.grad).all())
+        table.grad = None
+        del eager, graph
