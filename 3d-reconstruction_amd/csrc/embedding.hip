@@ -6,9 +6,9 @@
 //   1. the ids are sorted, stably, with their positions: by one workgroup in LDS up to EMB_SORT1 of them, else by a radix
 //      sort of three launches a digit.  The sort leaves most of the card idle, so its launches carry the zeros of the
 //      table along: workgroups behind those of the sort fill a share of it each.
-//   2. embed_runs_kernel cuts the sorted ids into pieces, one to a group of lanes as wide as a row.  A run of equal ids no
-//      longer than a piece is added up by the group in whose piece it starts, and stored; of a longer run each group adds
-//      what lies in its piece.
+//   2. embed_runs_kernel cuts the sorted ids into pieces, one to a group of lanes as wide as a row.  A short run of equal
+//      ids is added up by the group in whose piece it starts, and stored; of a long one each group adds what lies in its
+//      piece.
 //   3. embed_join_kernel adds the pieces of each long run.
 // Sums are held in fp32, taken in an order that the ids alone fix (no float atomics), and rounded once at the end.
 // Up to EMB_DIRECT ids need no sort: each workgroup picks the ids that fall among its rows of the table.  Nor does a table
@@ -32,8 +32,10 @@ constexpr int EMB_RADIX = 1 << EMB_RADIX_BITS;
 constexpr int EMB_ITEMS = 8;          // ids per thread and launch of the radix sort
 constexpr int EMB_TILE = EMB_THREADS * EMB_ITEMS;
 constexpr int EMB_JOIN_THREADS = 1024;
-constexpr int EMB_JOIN_PIECES = 16;   // pieces that a workgroup of the join looks at
-constexpr int EMB_PIECE_MAX = 64;
+constexpr int EMB_JOIN_PIECES = 256;  // pieces that a workgroup of the join looks at, at most
+constexpr int EMB_LONG_MAX = 64;
+constexpr int EMB_FLIGHT_RUNS = 8;    // rows a group has in flight there
+constexpr int EMB_JOIN_FLIGHT = 8;    // pieces a group of the join has in flight
 
 __device__ __forceinline__ int64_t emb_id(const void* ids, int id_bytes, int64_t i) {
   return id_bytes == 8 ? ((const int64_t*)ids)[i] : (int64_t)((const int32_t*)ids)[i];
@@ -89,7 +91,9 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_lookup_kernel(int64_t n, in
 struct EmbShape {
   int64_t n, V, vpr;  // ids, rows of the table, vectors per row
   int64_t gs;         // row stride of v_out in elements
-  int32_t G, rows_per, piece;
+  int32_t G, rows_per;
+  int32_t piece, longest;  // sorted ids of a group; of a run that one group adds up by itself (no fewer)
+  int32_t join;            // pieces that a workgroup of the join looks at
   float scale;
 };
 
@@ -386,28 +390,29 @@ __device__ __forceinline__ int64_t emb_lower(const uint32_t* keys, int64_t lo, i
   return lo;
 }
 
-// A group of G lanes takes the P sorted entries [i0, i1); its workgroup has their keys in LDS, with P more on both sides.
-// partial [pieces][2][D] fp32: what lies in the piece of the long run that started before it (slot 0), and of the long
-// run that starts in it (slot 1; there is one at most, and it goes on behind the piece).
+// A group of G lanes takes the P sorted entries [i0, i1); its workgroup has their keys in LDS, with
+// `longest` more on both sides.  partial [pieces][2][D] fp32: what lies in the piece of the long run that started before it (slot 0), and of the
+// long run that starts in it (slot 1; there is one at most, and it goes on behind the piece).
 template <typename T, int N>
 __global__ __launch_bounds__(EMB_THREADS) void embed_runs_kernel(EmbShape sh, const uint32_t* __restrict__ keys,
                                                                  const uint32_t* __restrict__ pos,
                                                                  const T* __restrict__ v_out, float* __restrict__ partial,
                                                                  T* __restrict__ v_table) {
   extern __shared__ uint32_t lds[];
-  const int P = sh.piece, groups = EMB_THREADS / sh.G, span = groups * P;
+  constexpr int FLIGHT = EMB_FLIGHT_RUNS;
+  const int P = sh.piece, M = sh.longest, groups = EMB_THREADS / sh.G, span = groups * P;
   const int64_t w0 = (int64_t)blockIdx.x * span;
-  uint32_t* lkey = lds;               // entries [w0 - P, w0 + span + P]
-  uint32_t* lpos = lds + span + 2 * P + 1;  // entries [w0, w0 + span + P)
-  for (int l = threadIdx.x; l < span + 2 * P + 1; l += EMB_THREADS) {
-    const int64_t e = w0 - P + l;
+  uint32_t* lkey = lds;                     // entries [w0 - M, w0 + span + M]
+  uint32_t* lpos = lds + span + 2 * M + 1;  // entries [w0, w0 + span + M)
+  for (int l = threadIdx.x; l < span + 2 * M + 1; l += EMB_THREADS) {
+    const int64_t e = w0 - M + l;
     lkey[l] = e < 0 ? 0xfffffffeu : e < sh.n ? keys[e] : 0xffffffffu;  // neither is a key
   }
-  for (int l = threadIdx.x; l < span + P; l += EMB_THREADS) lpos[l] = w0 + l < sh.n ? pos[w0 + l] : 0u;
+  for (int l = threadIdx.x; l < span + M; l += EMB_THREADS) lpos[l] = w0 + l < sh.n ? pos[w0 + l] : 0u;
   __syncthreads();
   const int g = threadIdx.x / sh.G;
   const int64_t vec = (int64_t)blockIdx.y * sh.G + (threadIdx.x & (sh.G - 1));
-  const uint32_t* key = lkey + P + g * P;  // key[0]: the piece's first entry
+  const uint32_t* key = lkey + M + g * P;  // key[0]: the piece's first entry
   const uint32_t* at = lpos + g * P;
   const int64_t i0 = w0 + (int64_t)g * P;
   if (i0 >= sh.n || vec >= sh.vpr) return;
@@ -418,37 +423,37 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_runs_kernel(EmbShape sh, co
   bool before = false;  // ... which belongs to a long run that started before the piece
   if (key[-1] == key[0]) {
     const uint32_t k = key[0];
-    const int s = key[-P] == k ? -P : (int)emb_lower(key, -P + 1, 0, k);
-    before = s == -P || key[s + P] == k;
+    const int s = key[-M] == k ? -M : (int)emb_lower(key, i0 < M ? -i0 : 1 - M, 0, k);
+    before = s == -M || key[s + M] == k;
     if (!before) a = (int)emb_lower(key, 0, i1, k + 1);  // a short run: the group where it starts has it
   }
   int b = i1;  // behind the last entry to add
   if (a < i1 && key[i1] == key[i1 - 1]) {
     const uint32_t k = key[i1 - 1];
     const int s = (int)emb_lower(key, a, i1, k);
-    if (!(before && s == 0) && key[s + P] != k) b = (int)emb_lower(key, i1, i1 + P, k + 1);  // a short run that starts here
+    if (!(before && s == 0) && key[s + M] != k) b = (int)emb_lower(key, i1, s + M, k + 1);  // a short run that starts here
   }
   const int64_t D = sh.vpr * N, col = vec * N, p = i0 / P;
   float acc[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) acc[k] = 0.f;
   int s = a;  // start of the run that is being added
-  for (int i = a; i < b; i += 4) {
+  for (int i = a; i < b; i += FLIGHT) {
     if (key[i] >= V) break;  // nothing but ids that select nothing from here on
-    float x[4][N];
+    Raw<T, N> raw[FLIGHT];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int e = i + u < b ? i + u : b - 1;
-      load_vec<T, N>(v_out + (int64_t)at[e] * sh.gs + col, x[u]);
-    }
+    for (int u = 0; u < FLIGHT; ++u)
+      raw[u] = load_raw<T, N>(v_out + (int64_t)at[i + u < b ? i + u : b - 1] * sh.gs + col);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < FLIGHT; ++u) {
       const int e = i + u;
       if (e < b && key[e] < V) {
+        float x[N];
+        unpack<T, N>(raw[u], x);
 #pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] += x[u][k];
+        for (int k = 0; k < N; ++k) acc[k] += x[k];
         if (e + 1 == b || key[e + 1] != key[e]) {
-          if (before || key[s + P] == key[s]) {
+          if (before || key[s + M] == key[s]) {
             float* to = partial + (2 * p + (before ? 0 : 1)) * D + col;
 #pragma unroll
             for (int k = 0; k < N; ++k) to[k] = acc[k];
@@ -465,53 +470,80 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_runs_kernel(EmbShape sh, co
   }
 }
 
-// A workgroup looks at EMB_JOIN_PIECES pieces; for each in which a long run starts it adds the run's pieces, its groups in
-// turn, and joins the groups in LDS, in their order.
+// Adds the partial sums of the pieces first, first + step, ... of the long run of `key` that starts in piece `start`.  A
+// piece is the run's exactly where its first entry is.  EMB_JOIN_FLIGHT are read at a time, whether they are or not: asking
+// first would cost a trip to memory for each.
+template <int N>
+__device__ __forceinline__ void emb_add_pieces(float (&acc)[N], const uint32_t* __restrict__ keys, int64_t pieces, int P,
+                                               uint32_t key, int64_t start, int64_t first, int64_t step,
+                                               const float* __restrict__ partial, int64_t D, int64_t col) {
+  bool more = true;
+  for (int64_t r = first; more; r += EMB_JOIN_FLIGHT * step) {
+    float x[EMB_JOIN_FLIGHT][N];
+    bool in[EMB_JOIN_FLIGHT];
+#pragma unroll
+    for (int u = 0; u < EMB_JOIN_FLIGHT; ++u) {
+      const int64_t c = r + u * step, d = c < pieces ? c : pieces - 1;
+      in[u] = c == start || (c < pieces && keys[d * P] == key);
+      const float* src = partial + (2 * d + (c == start ? 1 : 0)) * D + col;
+#pragma unroll
+      for (int k = 0; k < N; ++k) x[u][k] = src[k];
+    }
+#pragma unroll
+    for (int u = 0; u < EMB_JOIN_FLIGHT; ++u)
+#pragma unroll
+      for (int k = 0; k < N; ++k) acc[k] += in[u] ? x[u][k] : 0.f;
+    more = in[EMB_JOIN_FLIGHT - 1];
+  }
+}
+
+// A workgroup looks at some pieces for long runs that start in them.  One of its groups takes a run of few pieces; all take
+// one of many, and are joined in LDS, in their order.
 template <typename T, int N>
 __global__ __launch_bounds__(EMB_JOIN_THREADS) void embed_join_kernel(EmbShape sh, const uint32_t* __restrict__ keys,
                                                                       const float* __restrict__ partial,
                                                                       T* __restrict__ v_table) {
   __shared__ float lds[EMB_JOIN_THREADS * N];
-  __shared__ uint32_t near[(EMB_JOIN_PIECES + 1) * EMB_PIECE_MAX + 1];
-  __shared__ int64_t start[EMB_JOIN_PIECES];  // of the long run that starts in the piece, -1: none does
+  __shared__ int found[2][EMB_JOIN_PIECES], count[2];  // [longer ones]: pieces in which such a run starts
   const int P = sh.piece;
-  const int64_t p0 = (int64_t)blockIdx.x * EMB_JOIN_PIECES;
-  // near: the keys from the one before the pieces on, and P behind them
-  for (int l = threadIdx.x; l <= (EMB_JOIN_PIECES + 1) * P; l += EMB_JOIN_THREADS) {
-    const int64_t e = p0 * P - 1 + l;
-    near[l] = e < 0 ? 0xfffffffeu : e < sh.n ? keys[e] : 0xffffffffu;  // neither is a key
-  }
+  const int g = threadIdx.x / sh.G, groups = EMB_JOIN_THREADS / sh.G, few = groups / 2 > 32 ? groups / 2 : 32;
+  const int64_t p0 = (int64_t)blockIdx.x * sh.join, pieces = (sh.n + P - 1) / P;
+  if (threadIdx.x < 2) count[threadIdx.x] = 0;
   __syncthreads();
-  if (threadIdx.x < EMB_JOIN_PIECES) {
-    const uint32_t* key = near + 1 + threadIdx.x * P;  // key[0]: the piece's first entry
-    const uint32_t k = key[P - 1];
-    int64_t s = -1;
-    if (k < (uint32_t)sh.V && key[P] == k && key[-1] != k) {  // it starts here and goes on behind the piece
-      const int at = (int)emb_lower(key, 0, P, k);
-      if (key[at + P] == k) s = (p0 + threadIdx.x) * P + at;
+  if ((int)threadIdx.x < sh.join) {
+    const int64_t p = p0 + threadIdx.x, i0 = p * P, i1 = i0 + P;
+    if (i1 < sh.n) {
+      const uint32_t k = keys[i1 - 1];
+      // it goes on behind the piece, did not start before it, and is a long one
+      if (k < (uint32_t)sh.V && keys[i1] == k && !(i0 > 0 && keys[i0 - 1] == k)) {
+        const int64_t s = emb_lower(keys, i0, i1, k), far = p + few;
+        if (s + sh.longest < sh.n && keys[s + sh.longest] == k) {
+          const int longer = far * P < sh.n && keys[far * P] == k ? 1 : 0;
+          found[longer][atomicAdd(&count[longer], 1)] = threadIdx.x;  // (in any order: each run is added by itself)
+        }
+      }
     }
-    start[threadIdx.x] = s;
   }
   __syncthreads();
-  const int g = threadIdx.x / sh.G, groups = EMB_JOIN_THREADS / sh.G;
   const int64_t vec = (int64_t)blockIdx.y * sh.G + (threadIdx.x & (sh.G - 1));
-  const int64_t D = sh.vpr * N;
-  for (int q = 0; q < EMB_JOIN_PIECES; ++q) {
-    const int64_t s = start[q];
-    if (s < 0) continue;
-    const uint32_t key = near[1 + q * P + (int)(s - (p0 + q) * P)];
+  const int64_t D = sh.vpr * N, col = vec * N;
+  if (vec < sh.vpr)
+    for (int q = g; q < count[0]; q += groups) {
+      const int64_t p = p0 + found[0][q];
+      const uint32_t key = keys[p * P + P - 1];
+      float acc[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) acc[k] = 0.f;
+      emb_add_pieces<N>(acc, keys, pieces, P, key, p, p, 1, partial, D, col);
+      emb_store<T, N>(v_table + (int64_t)key * D + col, acc, sh.scale);
+    }
+  for (int q = 0; q < count[1]; ++q) {
+    const int64_t p = p0 + found[1][q];
+    const uint32_t key = keys[p * P + P - 1];
     float acc[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) acc[k] = 0.f;
-    if (vec < sh.vpr) {
-      for (int64_t r = p0 + q + g; r * P < sh.n; r += groups) {
-        const bool first = r == p0 + q;
-        if (!first && keys[r * P] != key) break;  // (a piece is the run's exactly where its first entry is)
-        const float* src = partial + (2 * r + (first ? 1 : 0)) * D + vec * N;
-#pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] += src[k];
-      }
-    }
+    if (vec < sh.vpr) emb_add_pieces<N>(acc, keys, pieces, P, key, p, p + g, groups, partial, D, col);
     for (int half = groups / 2; half > 0; half /= 2) {
       if (g >= half && g < 2 * half)
 #pragma unroll
@@ -522,7 +554,7 @@ __global__ __launch_bounds__(EMB_JOIN_THREADS) void embed_join_kernel(EmbShape s
         for (int k = 0; k < N; ++k) acc[k] += lds[k * EMB_JOIN_THREADS + half * sh.G + threadIdx.x];
       __syncthreads();
     }
-    if (g == 0 && vec < sh.vpr) emb_store<T, N>(v_table + (int64_t)key * D + vec * N, acc, sh.scale);
+    if (g == 0 && vec < sh.vpr) emb_store<T, N>(v_table + (int64_t)key * D + col, acc, sh.scale);
   }
 }
 
@@ -610,9 +642,10 @@ template <typename T, int N>
 __global__ __launch_bounds__(EMB_THREADS) void embed_direct_kernel(EmbShape sh, const void* __restrict__ ids, int id_bytes,
                                                                    const T* __restrict__ v_out, T* __restrict__ v_table) {
   static_assert(EMB_DIRECT <= EMB_THREADS, "a thread looks at one id");
-  __shared__ int hit_row[EMB_DIRECT];
+  __shared__ int hit_row[EMB_DIRECT], row_of[EMB_DIRECT];
   __shared__ uint32_t hit_pos[EMB_DIRECT];
   __shared__ int wave_hits[EMB_THREADS / 64];
+  __shared__ int start[EMB_ROWS_MAX + 1];
   const int64_t v0 = (int64_t)blockIdx.x * sh.rows_per;
   const int rows = (int)(sh.V - v0 < sh.rows_per ? sh.V - v0 : sh.rows_per);
   const int64_t id = (int64_t)threadIdx.x < sh.n ? emb_id(ids, id_bytes, threadIdx.x) : -1;
@@ -627,27 +660,43 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_direct_kernel(EmbShape sh, 
     if (w < wave) at += wave_hits[w];
     hits += wave_hits[w];
   }
-  if (mine) {
-    at += __popcll(ballot & ((1ull << lane) - 1ull));
-    hit_row[at] = (int)(id - v0);
-    hit_pos[at] = threadIdx.x;
-  }
-  __syncthreads();
   const int g = threadIdx.x / sh.G, groups = EMB_THREADS / sh.G;
   const int64_t vec = (int64_t)blockIdx.y * sh.G + (threadIdx.x & (sh.G - 1));
+  float acc[N];
+  if (hits > 0) {  // sorted by row, ids of a row in their order: each ranks itself
+    at += __popcll(ballot & ((1ull << lane) - 1ull));
+    if (mine) hit_row[at] = (int)(id - v0);
+    __syncthreads();
+    if (mine) {
+      const int r = (int)(id - v0);
+      int rank = 0;
+      for (int h = 0; h < hits; ++h) rank += hit_row[h] < r || (hit_row[h] == r && h < at);
+      row_of[rank] = r;
+      hit_pos[rank] = threadIdx.x;
+    }
+    __syncthreads();
+    for (int r = threadIdx.x; r <= rows; r += EMB_THREADS) {
+      int lo = 0, hi = hits;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (row_of[mid] < r) lo = mid + 1; else hi = mid;
+      }
+      start[r] = lo;
+    }
+    __syncthreads();
+  }
   if (vec >= sh.vpr) return;
   for (int r = g; r < rows; r += groups) {
-    float acc[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) acc[k] = 0.f;
-    for (int h = 0; h < hits; h += 8) {  // (all of the ids may be one row's)
+    const int s = hits > 0 ? start[r] : 0, e = hits > 0 ? start[r + 1] : 0;
+    for (int h = s; h < e; h += 8) {
       float x[8][N];
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (h + u < hits && hit_row[h + u] == r) load_vec<T, N>(v_out + (int64_t)hit_pos[h + u] * sh.gs + vec * N, x[u]);
+      for (int u = 0; u < 8; ++u) load_vec<T, N>(v_out + (int64_t)hit_pos[h + u < e ? h + u : e - 1] * sh.gs + vec * N, x[u]);
 #pragma unroll
       for (int u = 0; u < 8; ++u)
-        if (h + u < hits && hit_row[h + u] == r)
+        if (h + u < e)
 #pragma unroll
           for (int k = 0; k < N; ++k) acc[k] += x[u][k];
     }
@@ -683,9 +732,12 @@ struct EmbWorkspace {
 };
 
 // enough groups to fill the card first, then longer pieces: fewer partial sums of long runs
-static int emb_piece(int64_t n, int64_t D) { return n * D < ((int64_t)1 << 26) ? 16 : 64; }
+static int emb_piece(int64_t n, int64_t D) { return n * D < ((int64_t)1 << 26) ? 16 : EMB_LONG_MAX; }
 
-static bool emb_few(int64_t V, int64_t D) { return V <= EMB_FEW && D <= 65536; }
+// With many groups a run may keep one of them busy for longer, which saves the join: 1M ids on 65 x 16 and on 200000 x 16
+// fp32 take 91 and 142 us with runs of up to 16, 64 and 113 us with 64.  With few groups that one is what all wait for:
+// 16384 ids on 131072 x 1024 bf16 take 86 and 98 us.
+static int emb_longest(int64_t n, int64_t D) { return n >= 131072 ? EMB_LONG_MAX : emb_piece(n, D); }
 
 // Workgroups of the form for few rows: two on each CU, each with eight times as many ids as the table has rows, so that
 // the tables cost little next to what they were added up from.
@@ -694,10 +746,20 @@ static int64_t emb_few_blocks(int64_t n, int64_t V, int64_t D) {
   return std::max<int64_t>(1, std::min<int64_t>(ceil_div(512, tiles), n / (8 * V)));
 }
 
+// It is taken where it fills the card, or a thread has few rows to add: 5000 ids on 64 x 1024 fp32 take it 93 us, and
+// the sort 34 us; 1M ids on 64 x 16 take it 26 us, and the sort 68 us.
+static bool emb_few(int64_t n, int64_t V, int64_t D) {
+  if (V > EMB_FEW || D > 65536) return false;
+  int64_t Dp = 1;
+  while (Dp < EMB_THREADS && Dp < D) Dp <<= 1;
+  const int64_t blocks = emb_few_blocks(n, V, D);
+  return blocks * ceil_div(D, EMB_THREADS) >= 256 || ceil_div(n, blocks) * Dp <= 64 * EMB_THREADS;
+}
+
 static EmbWorkspace emb_workspace(int64_t n, int64_t V, int64_t D) {
   EmbWorkspace w = {};
   if (n <= EMB_DIRECT) return w;
-  if (emb_few(V, D)) {
+  if (emb_few(n, V, D)) {
     w.total = 4 * V * D * emb_few_blocks(n, V, D);
     return w;
   }
@@ -729,6 +791,8 @@ static int emb_sort(int64_t n, int64_t V, const void* ids, int32_t id_bytes, cha
     const dim3 grid(1 + emb_fill_blocks(fill, EMB_SORT1_THREADS)), block(EMB_SORT1_THREADS);
     if (n <= 4 * EMB_SORT1_THREADS)
       hipLaunchKernelGGL(embed_sort1_kernel<4>, grid, block, 0, s, (int)n, V, bits, ids, id_bytes, ka, pa, fill);
+    else if (n <= 8 * EMB_SORT1_THREADS)
+      hipLaunchKernelGGL(embed_sort1_kernel<8>, grid, block, 0, s, (int)n, V, bits, ids, id_bytes, ka, pa, fill);
     else
       hipLaunchKernelGGL(embed_sort1_kernel<16>, grid, block, 0, s, (int)n, V, bits, ids, id_bytes, ka, pa, fill);
     GS_CHECK_LAUNCH();
@@ -818,7 +882,7 @@ extern "C" int gs_embedding_bwd(int64_t n, int64_t V, int64_t D, int32_t dtype, 
   if (w.total > 0 && (!workspace || ((uintptr_t)workspace & 15))) return GS_ERR_INVALID_ARG;
   if (workspace_bytes < w.total) return GS_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
-  const int N = n > EMB_DIRECT && emb_few(V, D) ? 1 : emb_vec(D, size, v_out_stride, v_out, v_table);
+  const int N = n > EMB_DIRECT && emb_few(n, V, D) ? 1 : emb_vec(D, size, v_out_stride, v_out, v_table);
   EmbShape sh;
   sh.n = n; sh.V = V; sh.vpr = D / N; sh.gs = v_out_stride; sh.scale = scale;
   sh.G = 1;
@@ -839,7 +903,7 @@ extern "C" int gs_embedding_bwd(int64_t n, int64_t V, int64_t D, int32_t dtype, 
           GS_CHECK_LAUNCH();
           return GS_OK;
         }
-        if (emb_few(V, D)) {
+        if (emb_few(n, V, D)) {
           if constexpr (NV == 1) {
             EmbFew few{n, 0, v_out_stride, (int32_t)V, (int32_t)D, 1};
             while (few.Dp < EMB_THREADS && few.Dp < D) few.Dp <<= 1;
@@ -861,14 +925,16 @@ extern "C" int gs_embedding_bwd(int64_t n, int64_t V, int64_t D, int32_t dtype, 
         if (st != GS_OK) return st;
         sh.G = std::max(sh.G, 4);  // (keeps a workgroup's share of the sorted ids within 32 KiB of LDS)
         sh.piece = emb_piece(n, D);
+        sh.longest = emb_longest(n, D);
         float* partial = (float*)((char*)workspace + w.partial);
         const int64_t pieces = ceil_div(n, sh.piece);
+        sh.join = (int)std::min<int64_t>(std::max<int64_t>(pieces / 256, 16), EMB_JOIN_PIECES);
         const int span = EMB_THREADS / sh.G * sh.piece;
         hipLaunchKernelGGL((embed_runs_kernel<T, NV>), dim3((unsigned)ceil_div(n, span), (unsigned)tiles), dim3(EMB_THREADS),
-                           (2 * span + 3 * sh.piece + 1) * sizeof(uint32_t), s, sh, keys, pos, (const T*)v_out, partial,
+                           (2 * span + 3 * sh.longest + 1) * sizeof(uint32_t), s, sh, keys, pos, (const T*)v_out, partial,
                            (T*)v_table);
         GS_CHECK_LAUNCH();
-        hipLaunchKernelGGL((embed_join_kernel<T, NV>), dim3((unsigned)ceil_div(pieces, EMB_JOIN_PIECES), (unsigned)tiles),
+        hipLaunchKernelGGL((embed_join_kernel<T, NV>), dim3((unsigned)ceil_div(pieces, sh.join), (unsigned)tiles),
                            dim3(EMB_JOIN_THREADS), 0, s, sh, keys, partial, (T*)v_table);
         GS_CHECK_LAUNCH();
         return GS_OK;

@@ -23,6 +23,7 @@ constexpr int LP_BLOCKS_FWD = 1024;  // workgroups that the rows are cut into se
 constexpr int LP_BLOCKS_BWD = 8192;
 constexpr int LP_FLIGHT = 4;       // vectors a thread of the gradient has in flight
 constexpr int LP_ADD = 16;         // values added to the statistics at a time
+constexpr int LP_WAVE_LIST = 128;  // ... and a wave
 constexpr int LP_LIST = 1024;      // candidates for the top alternatives that a workgroup lists
 constexpr float LP_LOG2E = 1.44269504088896340736f;
 constexpr float LP_LOW = -1.0e4f;  // stands for -inf next to an exponential that is 0 there: 0 * LP_LOW is 0
@@ -80,13 +81,15 @@ __device__ __forceinline__ float lp_least(uint32_t order) { return lp_value(orde
 __device__ __forceinline__ uint64_t lp_key(float x, uint32_t j) { return ((uint64_t)lp_order(x) << 32) | (uint32_t)~j; }
 __device__ __forceinline__ uint32_t lp_key_index(uint64_t key) { return ~(uint32_t)key; }
 
-// A value that at least k lanes reach and that the k-th largest of them is not far above: its upper half, bit by bit, and
-// no further once no other lane reaches it (what is listed from it on is ranked anyway).
-__device__ __forceinline__ uint32_t lp_wave_kth(uint32_t v, int k) {
+// A value that at least k of the wave's values (M a lane) reach and that the k-th largest of them is not far above: its
+// upper half, bit by bit, and no further once just k reach it (what is listed from it on is ranked anyway).
+template <int M> __device__ __forceinline__ uint32_t lp_wave_kth(const uint32_t (&v)[M], int k) {
   uint32_t found = 0;
   for (int b = 31; b >= 16; --b) {
     const uint32_t want = found | (1u << b);
-    const int c = __popcll(__ballot(v >= want));
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < M; ++i) c += __popcll(__ballot(v[i] >= want));
     if (c >= k) found = want;
     if (c == k) break;
   }
@@ -225,8 +228,8 @@ template <typename T, int NV>
 __global__ __launch_bounds__(LP_THREADS) void label_wave_fwd_kernel(LpFwd a, const T* __restrict__ logits) {
   using Span = LpSpan<T>;
   constexpr int VE = Span::VE, NX = NV * VE + 1;
-  __shared__ uint64_t lists[LP_THREADS];
-  uint64_t* list = lists + (threadIdx.x & ~63u);
+  __shared__ uint64_t lists[LP_THREADS / 64][LP_WAVE_LIST];
+  uint64_t* list = lists[threadIdx.x >> 6];
   const int lane = threadIdx.x & 63;
   const int64_t waves = (int64_t)gridDim.x * (LP_THREADS / 64);
   for (int64_t r = (int64_t)blockIdx.x * (LP_THREADS / 64) + (threadIdx.x >> 6); r < a.rows; r += waves) {
@@ -261,10 +264,21 @@ __global__ __launch_bounds__(LP_THREADS) void label_wave_fwd_kernel(LpFwd a, con
       const int v = (i / VE) * 64 + lane;
       return v < sp.vecs ? sp.at(v) + i % VE : -1;
     };
-    // The k-th largest of the lanes' maxima is no larger than the k-th largest value: what is not below it is listed.
-    int listed = 65;
+    // The k-th largest of the lanes' maxima is no larger than the k-th largest value: what is not below it is listed.  For
+    // more than half as many alternatives as lanes that is too much, and the search goes over all values.
+    int listed = LP_WAVE_LIST + 1;
     if (st.s == st.s) {  // (NaN is above all, and no lane's maximum shows it: such rows go the long way)
-      const float least = lp_least(lp_wave_kth(lp_order(lane_max), a.top));
+      uint32_t order;
+      if (a.top <= 32) {
+        const uint32_t one[1] = {lp_order(lane_max)};
+        order = lp_wave_kth(one, a.top);
+      } else {
+        uint32_t all[NX];
+#pragma unroll
+        for (int i = 0; i < NX; ++i) all[i] = index(i) >= 0 ? lp_order(x[i]) : 0u;
+        order = lp_wave_kth(all, a.top);
+      }
+      const float least = lp_least(order);
       listed = 0;
 #pragma unroll
       for (int i = 0; i < NX; ++i) {
@@ -273,20 +287,19 @@ __global__ __launch_bounds__(LP_THREADS) void label_wave_fwd_kernel(LpFwd a, con
           const bool in = j >= 0 && x[i] >= least;
           const unsigned long long b = __ballot(in);
           const int at = listed + __popcll(b & ((1ull << lane) - 1ull));
-          if (in && at < 64) list[at] = lp_key(x[i], (uint32_t)j);
+          if (in && at < LP_WAVE_LIST) list[at] = lp_key(x[i], (uint32_t)j);
           listed += __popcll(b);
         }
       }
     }
-    if (listed <= 64) {  // each lane ranks one of them
+    if (listed <= LP_WAVE_LIST) {  // each lane ranks one or two of them
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
-      const uint64_t mine = lane < listed ? list[lane] : 0ull;
-      int rank = 0;
-      for (int i = 0; i < listed; ++i) rank += list[i] > mine;
-      if (lane < listed && rank < a.top) {
-        const uint32_t j = lp_key_index(mine);
-        lp_write_top(a, r, rank, j, lp_value((uint32_t)(mine >> 32)), st.m, ls);
+      for (int at = lane; at < listed; at += 64) {
+        const uint64_t mine = list[at];
+        int rank = 0;
+        for (int i = 0; i < listed; ++i) rank += list[i] > mine;
+        if (rank < a.top) lp_write_top(a, r, rank, lp_key_index(mine), lp_value((uint32_t)(mine >> 32)), st.m, ls);
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
@@ -363,7 +376,7 @@ template <typename T, typename F> __device__ __forceinline__ void lp_walk(const 
 
 struct LpShared {
   LpStat part[LP_THREADS / 64];
-  uint32_t least[LP_THREADS / 64];
+  uint32_t strips[LP_THREADS];
   uint64_t best[LP_THREADS / 64];
   int listed;
   uint64_t list[LP_LIST];
@@ -397,14 +410,13 @@ __device__ __forceinline__ void lp_block_top(const LpSpan<T>& sp, uint32_t j0, i
                                              LpShared& sh, F&& out) {
   int listed = LP_LIST + 1;
   if (!nan) {
-    const uint32_t kth = lp_wave_kth(lp_order(strip.m), top);
-    if ((threadIdx.x & 63) == 0) sh.least[threadIdx.x >> 6] = kth;
+    sh.strips[threadIdx.x] = lp_order(strip.m);
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
-    uint32_t order = sh.least[0];
+    uint32_t all[LP_THREADS / 64];  // (every wave searches for itself)
 #pragma unroll
-    for (int w = 1; w < LP_THREADS / 64; ++w) order = sh.least[w] > order ? sh.least[w] : order;
-    const float least = lp_least(order);
+    for (int w = 0; w < LP_THREADS / 64; ++w) all[w] = sh.strips[w * 64 + (threadIdx.x & 63)];
+    const float least = lp_least(lp_wave_kth(all, top));
     if (strip.m >= least)
       lp_walk(sp, [&](float x, int j) {
         if (x >= least) {
