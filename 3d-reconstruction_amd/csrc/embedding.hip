@@ -11,7 +11,7 @@
 //      piece.
 //   3. embed_join_kernel adds the pieces of each long run.
 // Sums are held in fp32, taken in an order that the ids alone fix (no float atomics), and rounded once at the end.
-// Up to EMB_DIRECT ids need no sort: each workgroup picks the ids that fall among its rows of the table.  Nor does a table
+// Up to EMB_DIRECT ids need no sort (but on a very large table): each workgroup picks the ids that fall among its rows of the table.  Nor does a table
 // of up to EMB_FEW rows, however many ids: it is added up in LDS.
 #include <algorithm>
 #include <type_traits>
@@ -727,6 +727,10 @@ static int emb_bits(int64_t V) {
 
 static int64_t emb_round(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
+// Tables beyond the Infinity Cache are better zeroed in one sweep: 64 ids on 131072 x 512 fp32 take 37 us directly and 45 us
+// sorted, on 131072 x 1024 141 and 119 us.
+static bool emb_direct(int64_t n, int64_t V, int64_t D) { return n <= EMB_DIRECT && V * D <= (int64_t)1 << 26; }
+
 struct EmbWorkspace {
   int64_t keys, pos, keys_b, pos_b, table, totals, partial, total;
 };
@@ -758,7 +762,7 @@ static bool emb_few(int64_t n, int64_t V, int64_t D) {
 
 static EmbWorkspace emb_workspace(int64_t n, int64_t V, int64_t D) {
   EmbWorkspace w = {};
-  if (n <= EMB_DIRECT) return w;
+  if (emb_direct(n, V, D)) return w;
   if (emb_few(n, V, D)) {
     w.total = 4 * V * D * emb_few_blocks(n, V, D);
     return w;
@@ -882,7 +886,7 @@ extern "C" int gs_embedding_bwd(int64_t n, int64_t V, int64_t D, int32_t dtype, 
   if (w.total > 0 && (!workspace || ((uintptr_t)workspace & 15))) return GS_ERR_INVALID_ARG;
   if (workspace_bytes < w.total) return GS_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
-  const int N = n > EMB_DIRECT && emb_few(n, V, D) ? 1 : emb_vec(D, size, v_out_stride, v_out, v_table);
+  const int N = !emb_direct(n, V, D) && emb_few(n, V, D) ? 1 : emb_vec(D, size, v_out_stride, v_out, v_table);
   EmbShape sh;
   sh.n = n; sh.V = V; sh.vpr = D / N; sh.gs = v_out_stride; sh.scale = scale;
   sh.G = 1;
@@ -894,7 +898,7 @@ extern "C" int gs_embedding_bwd(int64_t n, int64_t V, int64_t D, int32_t dtype, 
     return with_vec(size, N, [&](auto nv) {
       constexpr int NV = decltype(nv)::value;
       if constexpr (NV * (int)sizeof(T) <= 16) {
-        if (n <= EMB_DIRECT) {
+        if (emb_direct(n, V, D)) {
           // enough workgroups for 256 CUs first, then more rows each
           const int64_t per = std::max<int64_t>(ceil_div(V * tiles, 2048), EMB_THREADS / sh.G);
           sh.rows_per = (int)std::min<int64_t>(per, EMB_ROWS_MAX);
@@ -922,7 +926,7 @@ extern "C" int gs_embedding_bwd(int64_t n, int64_t V, int64_t D, int32_t dtype, 
         }
         const uint32_t *keys, *pos;
         const int st = emb_sort(n, V, ids, id_bytes, (char*)workspace, w, v_table, V * D * size, &keys, &pos, s);
-        if (st != GS_OK) return st;
+        if (st != GS_OK || n == 0) return st;  // (of no ids the zeros are all)
         sh.G = std::max(sh.G, 4);  // (keeps a workgroup's share of the sorted ids within 32 KiB of LDS)
         sh.piece = emb_piece(n, D);
         sh.longest = emb_longest(n, D);

@@ -264,6 +264,61 @@ def test_few_ids_of_one_row(gpu_device, n):
     _check(f"one row {n}", gpu_device, table, torch.full((n,), 77), 1.0, v_out)
 
 
+@pytest.mark.parametrize("n", [0, 1, 200])
+def test_few_ids_on_a_large_table(gpu_device, n):
+    from gsplat.prepass import embedding_lookup
+
+    dev, V, D = gpu_device, 70_000, 1001
+    g = torch.Generator().manual_seed(n)
+    ids = torch.randint(-1, V, (n,), generator=g)
+    ids[n // 2 :] = V - 1
+    up = torch.randn(n, D, generator=g)
+    table = torch.zeros(V, D, device=dev, requires_grad=True)
+    (v,) = torch.autograd.grad(embedding_lookup(table, ids.to(dev), 2.0), table, up.to(dev))
+    rows, where = torch.unique(ids[ids >= 0], return_inverse=True)
+    ref, size = (torch.zeros(len(rows), D, dtype=torch.float64).index_add_(0, where, t[ids >= 0]) * 2.0 for t in (up.double(), up.double().abs()))
+    assert_within(f"large {n}", v[rows.to(dev)], ref, (n + 1) * U * size + rounding(torch.float32, ref))
+    assert set((v != 0).any(1).nonzero()[:, 0].tolist()) == set(rows.tolist())
+
+
+def test_two_threads_on_streams_of_their_own(gpu_device):
+    import threading
+
+    from gsplat.gradients import clip_gradients
+    from gsplat.losses import label_log_probs
+    from gsplat.prepass import embedding_lookup
+
+    dev = gpu_device
+    table = torch.randn(4000, 40, device=dev)
+    ids = [torch.randint(0, 4000, (30_000,), device=dev) for _ in range(2)]
+
+    def step(k):
+        t = table.clone().requires_grad_(True)
+        got = label_log_probs(embedding_lookup(t, ids[k], 2.0), ids[k] % 40, top_k=3)
+        (v,) = torch.autograd.grad(got.log_prob.sum(), t)
+        clipped, norm = clip_gradients([v], 0.5)
+        return [got.log_prob, got.top_labels, v, clipped[0], norm]
+
+    want = [step(0), step(1)]
+    torch.cuda.synchronize()
+    seen = [[], []]
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream(dev)):
+            for _ in range(10):
+                seen[k].append(step(k))
+            torch.cuda.current_stream(dev).synchronize()
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for k in range(2):
+        assert len(seen[k]) == 10
+        assert all(torch.equal(a, b) for got in seen[k] for a, b in zip(got, want[k]))
+
+
 def test_captured_backward_next_to_an_eager_graph_is_refused(gpu_device):
     """An eager graph of the same leaf, made on another stream and still alive, would pull that stream into the capture."""
     from gsplat.losses import label_log_probs
