@@ -20,9 +20,13 @@ from . import _backend as B
 EPS = 1.0e-6  # added to the norm that max_norm is divided by
 
 
+def _listed(grads) -> List[Tensor]:
+    return [grads] if isinstance(grads, Tensor) else list(grads)  # (a tensor is one gradient, not its rows)
+
+
 def grad_norm(grads: Iterable[Tensor]) -> Tensor:
     """sqrt of the sum of squares over all tensors (fp32, bf16 and fp16, any mix) as a 0-d fp32 tensor on their device."""
-    return B.ops().grad_norm(list(grads))
+    return B.ops().grad_norm(_listed(grads))
 
 
 def clip_gradients(grads: Iterable[Tensor], max_norm: float, inplace: bool = False,
@@ -32,13 +36,14 @@ def clip_gradients(grads: Iterable[Tensor], max_norm: float, inplace: bool = Fal
     the same ones, which are neither read a second time nor written when the norm is within `max_norm`.  A NaN norm makes every gradient NaN and an infinite one
     makes the finite ones 0; `error_if_nonfinite` raises instead, before anything is changed (one host synchronisation and
     one more read of the gradients).  No two gradients may share memory when they are scaled in place."""
-    grads = list(grads)
+    grads = _listed(grads)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative or NaN, got {max_norm}")
     if error_if_nonfinite and not bool(torch.isfinite(grad_norm(grads))):
         raise RuntimeError("the total norm of the gradients is not finite: they are left as they are")
-    scaled, norm = B.ops().clip(grads, max_norm, EPS, inplace)
+    with B.timed("gs_grad_clip", grads[0].device if grads else None):
+        scaled, norm = B.ops().clip(grads, max_norm, EPS, inplace)
     return (grads if inplace else scaled), norm
 
 

@@ -322,5 +322,6 @@ def label_log_probs(logits: Tensor, labels: Tensor, top_k: int = 0) -> LabelLogP
     top_k = int(top_k)
     if not 0 <= top_k <= min(logits.shape[-1], 64):
         raise ValueError(f"top_k must be within 0..min(K, 64), got {top_k} for K = {logits.shape[-1]}")
-    log_prob, entropy, top, top_labels = B.ops().label_log_probs(logits, labels, top_k)
+    with B.timed("gs_label_log_probs_fwd", logits.device):
+        log_prob, entropy, top, top_labels = B.ops().label_log_probs(logits, labels, top_k)
     return LabelLogProbs(log_prob, entropy, top if top_k else None, top_labels if top_k else None)

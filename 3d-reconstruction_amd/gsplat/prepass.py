@@ -251,4 +251,5 @@ def embedding_lookup(table: Tensor, ids: Tensor, scale: float = 1.0, validate: b
     assert table.dim() == 2, f"table must be [V,D], got {tuple(table.shape)}"
     if validate and ids.numel() > 0 and not bool(((ids >= 0) & (ids < table.shape[0])).all()):
         raise IndexError(f"ids outside [0, {table.shape[0]})")
-    return B.ops().embedding_lookup(table, ids, scale)
+    with B.timed("gs_embedding_fwd", table.device):
+        return B.ops().embedding_lookup(table, ids, scale)

@@ -21,6 +21,8 @@
  *   gs_rasterize_fwd / _bwd         `rasterize_to_pixels` fwd/bwd incl. the "ED" normalisation (8a rows 8,9,10),
  *                                   call site R/models/trainers/base.py:393-408 and :772-787.
  *   gs_compact_visible              the CSR emission of `fully_fused_projection_packed`, packed=True.
+ *   gs_embedding_*, gs_label_log_probs_*, gs_grad_*   no callee of the reference: what a training step with learned codes
+ *                                   and class channels runs next to the rasterizer (last sections).
  *
  * Conventions: every pointer is a DEVICE pointer unless its name ends in `_host`; all tensors are
  * dense row-major fp32 / int32 / int64 as stated; `stream` is a hipStream_t passed as void*.
@@ -693,7 +695,7 @@ int gs_cube_texture_bwd(int64_t n, int32_t R, int32_t C, const float* dirs, cons
 int gs_embedding_fwd(int64_t n, int64_t V, int64_t D, int32_t dtype, const void* table, int64_t table_stride,
                      const void* ids, int32_t id_bytes, float scale, void* out, void* stream);
 /* v_table [V,D] (dense, written whole) = scale * the sum of the v_out rows (v_out_stride elements apart) of each id.
- * Sums in fp32, in an order the ids alone fix, rounded once.  n < 2^30, V < 2^31. */
+ * Sums in fp32, in an order the ids alone fix, rounded once.  n < 2^30, V < 2^31, D up to 4M vectors of 16 bytes. */
 int64_t gs_embedding_bwd_workspace_bytes(int64_t n, int64_t V, int64_t D);
 int gs_embedding_bwd(int64_t n, int64_t V, int64_t D, int32_t dtype, const void* ids, int32_t id_bytes,
                      const void* v_out, int64_t v_out_stride, float scale, void* workspace /* 16-B aligned */,

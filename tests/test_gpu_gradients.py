@@ -206,3 +206,39 @@ def test_refusals_on_the_device(gpu_device):
         clip_gradients([flat.to_sparse()], 1.0)
     with pytest.raises(RuntimeError, match="no CPU path|different devices"):
         clip_gradients([flat, flat.cpu()], 1.0)
+
+
+def test_outputs_are_ordinary_tensors(gpu_device):
+    """The small ones share an allocation: nothing else about them differs."""
+    import io
+
+    from gsplat.gradients import clip_gradients, grad_norm
+
+    dev = gpu_device
+    grads = [torch.randn(7, device=dev), torch.randn(3, 5, device=dev).bfloat16(), torch.randn(4, 6, device=dev).t(), torch.empty(0, device=dev),
+             torch.randn(200_000, device=dev)]
+    out, norm = clip_gradients(grads, 1e-3)
+    assert all(o.data_ptr() % 512 == 0 and o.stride() == g.stride() and not o.requires_grad and not o._is_view() for o, g in zip(out, grads))
+    keep = [o.clone() for o in out]
+    version = out[1]._version
+    out[0].zero_()
+    assert out[1]._version == version
+    out[0] = keep[0].clone()
+    assert all(torch.equal(a, b) for a, b in zip(out, keep))
+    leaf = out[1].requires_grad_(True)
+    (leaf.float() * 2).sum().backward()
+    assert bool((leaf.grad == 2).all())
+    leaf.detach().mul_(0)
+    assert torch.equal(out[2], keep[2])
+    buf = io.BytesIO()
+    torch.save(out[2], buf)
+    buf.seek(0)
+    assert torch.equal(torch.load(buf, weights_only=True), keep[2])
+    one, n = clip_gradients(grads[4], 1.0)  # a tensor is one gradient
+    assert len(one) == 1 and one[0].shape == grads[4].shape and torch.equal(n, grad_norm(grads[4]))
+    other = torch.cuda.Stream(dev)
+    with torch.cuda.stream(other):  # the pool goes back to its stream's memory when the last of them is gone
+        del out, leaf
+        again, _ = clip_gradients(grads, 1e-3)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(again, keep))
