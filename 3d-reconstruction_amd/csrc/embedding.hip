@@ -12,7 +12,7 @@
 //   3. embed_join_kernel adds the pieces of each long run.
 // Sums are held in fp32, taken in an order that the ids alone fix (no float atomics), and rounded once at the end.
 // Up to EMB_DIRECT ids need no sort (but on a very large table): each workgroup picks the ids that fall among its rows.
-// Nor does a table of up to EMB_FEW rows, however many ids: it is added up in LDS.
+// Nor does a table of few and short rows, however many ids: it is added up in LDS.
 #include <algorithm>
 #include <type_traits>
 
@@ -23,7 +23,7 @@ namespace gs {
 constexpr int EMB_THREADS = 256;
 constexpr int EMB_FLIGHT = 4;         // rows a thread of the lookup has in flight
 constexpr int EMB_DIRECT = 256;
-constexpr int EMB_FEW = 64;           // rows of a table that fits LDS once for each row a workgroup reads at a time
+constexpr int EMB_FEW = 64;           // rows of a table that LDS holds once for each row that a workgroup reads at a time
 constexpr int EMB_ROWS_MAX = 256;     // rows of the table per workgroup of the direct form
 constexpr int EMB_SORT1 = 16384;      // ids that one workgroup sorts in LDS
 constexpr int EMB_SORT1_THREADS = 1024;
@@ -566,14 +566,13 @@ __global__ __launch_bounds__(EMB_JOIN_THREADS) void embed_join_kernel(EmbShape s
   }
 }
 
-// ---- few rows (V <= EMB_FEW): no sort.  256 threads read 256 values at a time, a column each (a row of D <= 128 columns
-// leaves room for several rows), and add them to a table in LDS that belongs to the thread's place among those rows: no
-// two threads meet in a word.  Equal ids in succession, the rule where Gaussians lie instance by instance, add up in a
+// ---- few rows (V <= EMB_FEW, of D <= 128 columns): no sort.  256 threads read 256 values at a time, several rows, a column
+// each, and add them to a table in LDS that belongs to the thread's place among those rows: no two threads meet in a word.  Equal ids in succession, the rule where Gaussians lie instance by instance, add up in a
 // register first.  The tables of a workgroup are added up, in their order, and embed_few_join_kernel adds the workgroups'.
 // 1M x 16 fp32 on 64 rows: 24 + 4 us (3.0 TB/s; LDS leaves a CU eight waves), against 64 us by the sort.
 struct EmbFew {
   int64_t n, per, gs;   // ids, ids of a workgroup, row stride of v_out
-  int32_t V, D, Dp;     // Dp: columns of a workgroup, a power of two
+  int32_t V, D, Dp;     // Dp: D rounded up to a power of two
 };
 
 template <typename T>
@@ -581,11 +580,11 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_few_kernel(EmbFew sh, const
                                                                 const T* __restrict__ v_out, float* __restrict__ partial) {
   extern __shared__ float tables[];  // [256 / Dp][V][Dp]
   constexpr int U = 16;
-  const int S = EMB_THREADS / sh.Dp, c = threadIdx.x & (sh.Dp - 1), col = blockIdx.y * sh.Dp + c;
+  const int S = EMB_THREADS / sh.Dp, col = threadIdx.x & (sh.Dp - 1);
   for (int e = threadIdx.x; e < sh.V * EMB_THREADS; e += EMB_THREADS) tables[e] = 0.f;
   __syncthreads();
   if (col < sh.D) {
-    float* mine = tables + threadIdx.x / sh.Dp * sh.V * sh.Dp + c;
+    float* mine = tables + threadIdx.x / sh.Dp * sh.V * sh.Dp + col;
     const int64_t r0 = blockIdx.x * sh.per, r1 = r0 + sh.per < sh.n ? r0 + sh.per : sh.n;
     int last = -1;  // -1: no row
     float acc = 0.f;
@@ -619,7 +618,7 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_few_kernel(EmbFew sh, const
   __syncthreads();
   const int size = sh.V * sh.Dp;
   for (int e = threadIdx.x; e < size; e += EMB_THREADS) {
-    const int to = blockIdx.y * sh.Dp + (e & (sh.Dp - 1));
+    const int to = e & (sh.Dp - 1);
     if (to >= sh.D) continue;
     float sum = tables[e];
     for (int k = 1; k < S; ++k) sum += tables[k * size + e];
@@ -745,36 +744,31 @@ struct EmbWorkspace {
   int64_t keys, pos, keys_b, pos_b, table, totals, partial, total;
 };
 
-// enough groups to fill the card first, then longer pieces: fewer partial sums of long runs
-static int emb_piece(int64_t n, int64_t D) { return n * D < ((int64_t)1 << 26) ? 16 : EMB_LONG_MAX; }
+// enough groups to fill the card first, then longer pieces: fewer partial sums of long runs (embed_runs_kernel with pieces of
+// 4 and of 16: 16384 ids on 5000 x 16 fp32 8.2 and 13.8 us, 1000 ids 5.7 and 9.8 us)
+static int emb_piece(int64_t n, int64_t D) {
+  return n * D < ((int64_t)1 << 20) ? 4 : n * D < ((int64_t)1 << 26) ? 16 : EMB_LONG_MAX;
+}
 
 // With many groups a run may keep one of them busy for longer, which saves the join: 1M ids on 65 x 16 and on 200000 x 16
 // fp32 take 91 and 142 us with runs of up to 16, 64 and 113 us with 64.  With few groups that one is what all wait for:
 // 16384 ids on 131072 x 1024 bf16 take 86 and 98 us.
-static int emb_longest(int64_t n, int64_t D) { return n >= 131072 ? EMB_LONG_MAX : emb_piece(n, D); }
+static int emb_longest(int64_t n, int64_t D) { return n >= 131072 ? EMB_LONG_MAX : std::max(16, emb_piece(n, D)); }
 
-// Workgroups of the form for few rows: two on each CU, each with eight times as many ids as the table has rows, so that
-// the tables cost little next to what they were added up from.
-static int64_t emb_few_blocks(int64_t n, int64_t V, int64_t D) {
-  const int64_t tiles = ceil_div(D, EMB_THREADS);
-  return std::max<int64_t>(1, std::min<int64_t>(ceil_div(512, tiles), n / (8 * V)));
-}
+// The form for few rows is taken where a workgroup reads two rows or more at a time: gradients alone, by it and by the sort,
+// 1M ids on 64 x 16 fp32 31 and 67 us, 38358 on 6 x 36 10 and 29, 20000 on 64 x 64 17 and 35, 300 on 64 x 64 16 and 16; but
+// 100000 on 64 x 256 55 and 48, on 64 x 1024 143 and 74.
+static bool emb_few(int64_t V, int64_t D) { return V <= EMB_FEW && D <= EMB_THREADS / 2; }
 
-// It is taken where it fills the card, or a thread has few rows to add: 5000 ids on 64 x 1024 fp32 take it 93 us, and
-// the sort 34 us; 1M ids on 64 x 16 take it 26 us, and the sort 68 us.
-static bool emb_few(int64_t n, int64_t V, int64_t D) {
-  if (V > EMB_FEW || D > 65536) return false;
-  int64_t Dp = 1;
-  while (Dp < EMB_THREADS && Dp < D) Dp <<= 1;
-  const int64_t blocks = emb_few_blocks(n, V, D);
-  return blocks * ceil_div(D, EMB_THREADS) >= 256 || ceil_div(n, blocks) * Dp <= 64 * EMB_THREADS;
-}
+// Its workgroups: two on each CU, each with twice as many ids as the table has rows or more, so that writing and adding up
+// their tables costs no more than reading the rows.
+static int64_t emb_few_blocks(int64_t n, int64_t V) { return std::max<int64_t>(1, std::min<int64_t>(512, n / (2 * V))); }
 
 static EmbWorkspace emb_workspace(int64_t n, int64_t V, int64_t D) {
   EmbWorkspace w = {};
   if (emb_direct(n, V, D)) return w;
-  if (emb_few(n, V, D)) {
-    w.total = 4 * V * D * emb_few_blocks(n, V, D);
+  if (emb_few(V, D)) {
+    w.total = 4 * V * D * emb_few_blocks(n, V);
     return w;
   }
   const int64_t list = emb_round(4 * n), blocks = ceil_div(n, EMB_TILE);
@@ -896,7 +890,7 @@ extern "C" int gs_embedding_bwd(int64_t n, int64_t V, int64_t D, int32_t dtype, 
   if (w.total > 0 && (!workspace || ((uintptr_t)workspace & 15))) return GS_ERR_INVALID_ARG;
   if (workspace_bytes < w.total) return GS_ERR_WORKSPACE;
   hipStream_t s = (hipStream_t)stream;
-  const int N = !emb_direct(n, V, D) && emb_few(n, V, D) ? 1 : emb_vec(D, size, v_out_stride, v_out, v_table);
+  const int N = !emb_direct(n, V, D) && emb_few(V, D) ? 1 : emb_vec(D, size, v_out_stride, v_out, v_table);
   EmbShape sh;
   sh.n = n; sh.V = V; sh.vpr = D / N; sh.gs = v_out_stride; sh.scale = scale;
   sh.G = 1;
@@ -917,13 +911,13 @@ extern "C" int gs_embedding_bwd(int64_t n, int64_t V, int64_t D, int32_t dtype, 
           GS_CHECK_LAUNCH();
           return GS_OK;
         }
-        if (emb_few(n, V, D)) {
+        if (emb_few(V, D)) {
           if constexpr (NV == 1) {
             EmbFew few{n, 0, v_out_stride, (int32_t)V, (int32_t)D, 1};
-            while (few.Dp < EMB_THREADS && few.Dp < D) few.Dp <<= 1;
-            const int64_t blocks = emb_few_blocks(n, V, D);
+            while (few.Dp < D) few.Dp <<= 1;
+            const int64_t blocks = emb_few_blocks(n, V);
             few.per = ceil_div(n, blocks);
-            hipLaunchKernelGGL(embed_few_kernel<T>, dim3((unsigned)blocks, (unsigned)ceil_div(D, few.Dp)), dim3(EMB_THREADS),
+            hipLaunchKernelGGL(embed_few_kernel<T>, dim3((unsigned)blocks), dim3(EMB_THREADS),
                                V * EMB_THREADS * sizeof(float), s, few, ids, id_bytes, (const T*)v_out, (float*)workspace);
             GS_CHECK_LAUNCH();
             const int words = (int)(V * D);
