@@ -82,17 +82,22 @@ __device__ __forceinline__ float lp_least(uint32_t order) { return lp_value(orde
 __device__ __forceinline__ uint64_t lp_key(float x, uint32_t j) { return ((uint64_t)lp_order(x) << 32) | (uint32_t)~j; }
 __device__ __forceinline__ uint32_t lp_key_index(uint64_t key) { return ~(uint32_t)key; }
 
-// A value that at least k of the wave's values (M a lane) reach and that the k-th largest of them is not far above: its
-// upper half, bit by bit, and no further once just k reach it (what is listed from it on is ranked anyway).
-template <int M> __device__ __forceinline__ uint32_t lp_wave_kth(const uint32_t (&v)[M], int k) {
+// A value that at least k of the wave's values (M a lane) reach, `reach` of them, and that the k-th largest is not far
+// above: its upper half, bit by bit, and no further once just k reach it (what is listed from it on is ranked anyway).
+// EXACT: the k-th largest itself.
+template <bool EXACT, int M> __device__ __forceinline__ uint32_t lp_wave_kth(const uint32_t (&v)[M], int k, int& reach) {
   uint32_t found = 0;
-  for (int b = 31; b >= 16; --b) {
+  reach = 64 * M;
+  for (int b = 31; b >= (EXACT ? 0 : 16); --b) {
     const uint32_t want = found | (1u << b);
     int c = 0;
 #pragma unroll
     for (int i = 0; i < M; ++i) c += __popcll(__ballot(v[i] >= want));
-    if (c >= k) found = want;
-    if (c == k) break;
+    if (c >= k) {
+      found = want;
+      reach = c;
+    }
+    if (!EXACT && c == k) break;
   }
   return found;
 }
@@ -227,10 +232,75 @@ __global__ __launch_bounds__(64) void label_small_fwd_kernel(LpFwd a, uint32_t m
 
 // -------------------------------------------------------------------------------------------- up to LP_WAVE classes
 // A wave holds a row in registers: NV vectors a lane and one extra value.  Read once, whatever is asked for.
-// 8191 x 1000 fp32 with the five best 11 us (3.0 TB/s), a quarter of it for the alternatives; bound by instructions, five
-// waves on a SIMD (forced to eight, with values spilled, 16 us).
+// 8191 x 1000 fp32 with the five best 11 us (3.0 TB/s), a quarter of it for the alternatives, and 19 us where just three
+// classes are not ruled out; bound by instructions, six waves on a SIMD (forced to eight, with values spilled, 16 us).  Four
+// at least: 8191 x 2048 bf16 with the twenty best 20 us, three waves 25.
+// f(value, index) over thread t's strip: every LANES-th vector
+template <int LANES, typename T, typename F> __device__ __forceinline__ void lp_walk(const LpSpan<T>& sp, int t, F&& f) {
+  constexpr int VE = LpSpan<T>::VE;
+  for (int v = t; v < sp.vecs; v += LANES) {
+    float x[VE];
+    sp.load(v, x);
+#pragma unroll
+    for (int k = 0; k < VE; ++k) f(x[k], sp.at(v) + k);
+  }
+  const int ex = sp.extra(t);
+  if (ex >= 0) f((float)sp.x[ex], ex);
+}
+
+// Rows of many equal values (classes ruled out): lists what is above `tie` and, in the order of their indices, the values
+// that equal it until there are `top`.  Returns how many are listed; more than LP_WAVE_LIST: too many are above it.  The row
+// is read again, out of the caches: the registers that would keep it until here are better spent on more waves.
+template <typename T>
+__device__ __forceinline__ int lp_wave_ties(const LpSpan<T>& sp, int lane, int top, float tie, uint64_t* __restrict__ list) {
+  constexpr int VE = LpSpan<T>::VE;
+  const unsigned long long lower = (1ull << lane) - 1ull;
+  int listed = 0;
+  auto one = [&](bool in, float x, int j) {
+    const unsigned long long b = __ballot(in);
+    const int at = listed + __popcll(b & lower);
+    if (in && at < LP_WAVE_LIST) list[at] = lp_key(x, (uint32_t)j);
+    listed += __popcll(b);
+  };
+  const int ex = sp.extra(lane);
+  const float x_ex = ex >= 0 ? (float)sp.x[ex] : -INFINITY;
+  one(x_ex > tie, x_ex, ex);
+  for (int v0 = 0; v0 < sp.vecs; v0 += 64) {
+    float x[VE];
+#pragma unroll
+    for (int k = 0; k < VE; ++k) x[k] = -INFINITY;
+    if (v0 + lane < sp.vecs) sp.load(v0 + lane, x);
+#pragma unroll
+    for (int k = 0; k < VE; ++k) one(x[k] > tie, x[k], sp.at(v0 + lane) + k);
+  }
+  if (listed > LP_WAVE_LIST - GS_LABEL_TOP_MAX) return LP_WAVE_LIST + 1;
+  if (listed >= top) return listed;
+  one(ex >= 0 && ex < sp.head && x_ex == tie, tie, ex);  // (no more than LP_WAVE_LIST in all: the head is short)
+  for (int v0 = 0; v0 < sp.vecs && listed < top; v0 += 64) {
+    float x[VE];
+    const bool there = v0 + lane < sp.vecs;
+    if (there) sp.load(v0 + lane, x);
+    unsigned long long b[VE];
+    int at = listed;
+#pragma unroll
+    for (int k = 0; k < VE; ++k) {
+      b[k] = __ballot(there && x[k] == tie);
+      at += __popcll(b[k] & lower);
+      listed += __popcll(b[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < VE; ++k)
+      if ((b[k] >> lane) & 1ull) {
+        if (at < top) list[at] = lp_key(tie, (uint32_t)(sp.at(v0 + lane) + k));
+        ++at;
+      }
+  }
+  if (listed < top) one(ex >= sp.head && x_ex == tie, tie, ex);
+  return listed < top ? listed : top;
+}
+
 template <typename T, int NV>
-__global__ __launch_bounds__(LP_THREADS) void label_wave_fwd_kernel(LpFwd a, const T* __restrict__ logits) {
+__global__ __launch_bounds__(LP_THREADS, 4) void label_wave_fwd_kernel(LpFwd a, const T* __restrict__ logits) {
   using Span = LpSpan<T>;
   constexpr int VE = Span::VE, NX = NV * VE + 1;
   __shared__ uint64_t lists[LP_THREADS / 64][LP_WAVE_LIST];
@@ -274,14 +344,15 @@ __global__ __launch_bounds__(LP_THREADS) void label_wave_fwd_kernel(LpFwd a, con
     int listed = LP_WAVE_LIST + 1;
     if (st.s == st.s) {  // (NaN is above all, and no lane's maximum shows it: such rows go the long way)
       uint32_t order;
+      int reach;
       if (a.top <= 32) {
         const uint32_t one[1] = {lp_order(lane_max)};
-        order = lp_wave_kth(one, a.top);
+        order = lp_wave_kth<false>(one, a.top, reach);
       } else {
         uint32_t all[NX];
 #pragma unroll
         for (int i = 0; i < NX; ++i) all[i] = index(i) >= 0 ? lp_order(x[i]) : 0u;
-        order = lp_wave_kth(all, a.top);
+        order = lp_wave_kth<false>(all, a.top, reach);
       }
       const float least = lp_least(order);
       listed = 0;
@@ -296,6 +367,10 @@ __global__ __launch_bounds__(LP_THREADS) void label_wave_fwd_kernel(LpFwd a, con
           listed += __popcll(b);
         }
       }
+      if (listed > LP_WAVE_LIST) {
+        const uint32_t one[1] = {lp_order(lane_max)};
+        listed = lp_wave_ties(sp, lane, a.top, lp_least(lp_wave_kth<true>(one, a.top, reach)), list);
+      }
     }
     if (listed <= LP_WAVE_LIST) {  // each lane ranks one or two of them
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -308,16 +383,14 @@ __global__ __launch_bounds__(LP_THREADS) void label_wave_fwd_kernel(LpFwd a, con
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
-    } else {  // many equal values, or NaN: one alternative after another
+    } else {  // NaN, or too many values above many equal ones: one alternative after another
       uint64_t below = ~0ull;
       for (int t = 0; t < a.top; ++t) {
         uint64_t best = 0;
-#pragma unroll
-        for (int i = 0; i < NX; ++i) {
-          const int j = index(i);
-          const uint64_t k = j >= 0 ? lp_key(x[i], (uint32_t)j) : 0ull;
+        lp_walk<64>(sp, lane, [&](float f, int j) {
+          const uint64_t k = lp_key(f, (uint32_t)j);
           if (k < below && k > best) best = k;
-        }
+        });
         best = wave_max_all(best);
         below = best;
         const uint32_t j = lp_key_index(best);
@@ -331,10 +404,12 @@ __global__ __launch_bounds__(LP_THREADS) void label_wave_fwd_kernel(LpFwd a, con
 // A workgroup reads a segment of a row (all of it when there are rows enough to fill the card), four vectors a thread in
 // flight.  A thread's strip is every 256th vector; its maximum comes out of the statistics for nothing, and the k-th
 // largest of a wave's strip maxima is no larger than the k-th largest value: only strips that reach it are read again,
-// and what they hold from it on is listed and ranked.  Rows whose list overflows (very many equal values) or that hold
-// NaN take the alternatives one by one, each thread keeping its strip's best and reading the strip again when it won.
+// and what they hold from it on is listed and ranked.  Where many strips reach it (equal logits, classes ruled out) the
+// list takes what is above the k-th largest maximum and the first values that equal it.  Rows whose list overflows all the
+// same or that hold NaN take the alternatives one by one, each thread keeping its strip's best and reading the strip again
+// when it won.
 // 2048 x 100277 bf16 74 us (5.5 TB/s); one row of 131072 bf16 with its eight best 5.6 us in 64 segments and 3.4 us to join
-// them; 2048 x 131072 183 us with the twenty best, and 2.5 ms where all logits are equal.
+// them; 2048 x 131072 130 us with the twenty best, 109 us where all logits are equal (2.5 ms one by one).
 struct LpPart {  // of one segment
   float m, s, w, pad;
 };
@@ -368,24 +443,12 @@ template <typename T> __device__ __forceinline__ LpStat lp_strip(const LpSpan<T>
   return st;
 }
 
-// f(value, index) over the thread's strip
-template <typename T, typename F> __device__ __forceinline__ void lp_walk(const LpSpan<T>& sp, F&& f) {
-  constexpr int VE = LpSpan<T>::VE;
-  for (int v = threadIdx.x; v < sp.vecs; v += LP_THREADS) {
-    float x[VE];
-    sp.load(v, x);
-#pragma unroll
-    for (int k = 0; k < VE; ++k) f(x[k], sp.at(v) + k);
-  }
-  const int ex = sp.extra(threadIdx.x);
-  if (ex >= 0) f((float)sp.x[ex], ex);
-}
-
 struct LpShared {
   LpStat part[LP_THREADS / 64];
   uint32_t strips[LP_THREADS];
   uint64_t best[LP_THREADS / 64];
-  int listed;
+  uint8_t who[LP_THREADS];  // strips that are walked together, `found` of them
+  int listed, found;
   uint64_t list[LP_LIST];
 };
 
@@ -411,6 +474,90 @@ __device__ __forceinline__ uint64_t lp_block_max(uint64_t v, uint64_t* lds) {
   return m;
 }
 
+// f(value, index) over the strips of the threads that want theirs walked, all threads at the same number of vectors: a few
+// threads with a long strip each would keep the workgroup waiting (2048 x 131072 bf16 with the twenty best 181 us, so 130;
+// 2048 x 100277 with the five best 117 and 80 us).  sh.found is 0 before.
+template <typename T, typename F>
+__device__ __forceinline__ void lp_walk_some(const LpSpan<T>& sp, bool mine, LpShared& sh, F&& f) {
+  constexpr int VE = LpSpan<T>::VE;
+  if (mine) {
+    sh.who[atomicAdd(&sh.found, 1)] = (uint8_t)threadIdx.x;
+    const int ex = sp.extra(threadIdx.x);
+    if (ex >= 0) f((float)sp.x[ex], ex);
+  }
+  __syncthreads();
+  const uint32_t strips = (uint32_t)sh.found, items = strips * (uint32_t)((sp.vecs + LP_THREADS - 1) / LP_THREADS);
+  for (uint32_t q = threadIdx.x; q < items; q += LP_THREADS) {  // (four at a time: no faster)
+    const uint32_t i = q / strips;
+    const int v = (int)(i * LP_THREADS + sh.who[q - i * strips]);
+    if (v < sp.vecs) {
+      float x[VE];
+      sp.load(v, x);
+#pragma unroll
+      for (int k = 0; k < VE; ++k) f(x[k], sp.at(v) + k);
+    }
+  }
+  __syncthreads();
+}
+
+// Lists what is above `kth` and, in the order of their indices, the values that equal it until there are `top`.  Returns
+// how many are listed; more than LP_LIST: too many are above it.
+template <typename T>
+__device__ __forceinline__ int lp_block_ties(const LpSpan<T>& sp, uint32_t j0, int top, uint32_t strip, uint32_t kth,
+                                             LpShared& sh) {
+  constexpr int VE = LpSpan<T>::VE, WAVES = LP_THREADS / 64;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  __syncthreads();
+  if (t == 0) sh.listed = sh.found = 0;
+  __syncthreads();
+  lp_walk_some(sp, strip > kth, sh, [&](float x, int j) {
+    if (lp_order(x) > kth) {
+      const int at = atomicAdd(&sh.listed, 1);
+      if (at < LP_LIST) sh.list[at] = lp_key(x, j0 + (uint32_t)j);
+    }
+  });
+  int have = sh.listed, round = 0;
+  if (have > LP_LIST - GS_LABEL_TOP_MAX) return LP_LIST + 1;
+  if (have >= top) return have;
+  // bits: which of the thread's values from index j on equal it, the threads in the order of their values
+  auto take = [&](uint32_t bits, int j) {
+    uint32_t* sums = sh.strips + (round++ & 1) * WAVES;
+    const int own = __popc(bits);
+    int at = own;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int before = __shfl_up(at, o);
+      if (lane >= o) at += before;
+    }
+    if (lane == 63) sums[wave] = (uint32_t)at;
+    __syncthreads();
+    at += have - own;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      if (w < wave) at += (int)sums[w];
+      have += (int)sums[w];
+    }
+    for (; bits && at < top; bits &= bits - 1) sh.list[at++] = ((uint64_t)kth << 32) | (uint32_t)~(j0 + (uint32_t)(j + __ffs((int)bits) - 1));
+  };
+  take(t < sp.head && lp_order((float)sp.x[t]) == kth ? 1u : 0u, t);
+  for (int v0 = 0; v0 < sp.vecs && have < top; v0 += LP_THREADS) {
+    uint32_t bits = 0;
+    if (v0 + t < sp.vecs) {
+      float x[VE];
+      sp.load(v0 + t, x);
+#pragma unroll
+      for (int k = 0; k < VE; ++k) bits |= lp_order(x[k]) == kth ? 1u << k : 0u;
+    }
+    take(bits, sp.at(v0 + t));
+  }
+  if (have < top) {
+    const int j = sp.at(sp.vecs) + t;
+    take(j < sp.n && lp_order((float)sp.x[j]) == kth ? 1u : 0u, j);
+  }
+  __syncthreads();
+  return have < top ? have : top;
+}
+
 // out(rank, key) for the segment's largest `top` values, in any order of ranks; j0 = index of its first value
 template <typename T, typename F>
 __device__ __forceinline__ void lp_block_top(const LpSpan<T>& sp, uint32_t j0, int top, const LpStat& strip, bool nan,
@@ -418,21 +565,26 @@ __device__ __forceinline__ void lp_block_top(const LpSpan<T>& sp, uint32_t j0, i
   int listed = LP_LIST + 1;
   if (!nan) {
     sh.strips[threadIdx.x] = lp_order(strip.m);
-    if (threadIdx.x == 0) sh.listed = 0;
+    if (threadIdx.x == 0) sh.listed = sh.found = 0;
     __syncthreads();
     uint32_t all[LP_THREADS / 64];  // (every wave searches for itself)
 #pragma unroll
     for (int w = 0; w < LP_THREADS / 64; ++w) all[w] = sh.strips[w * 64 + (threadIdx.x & 63)];
-    const float least = lp_least(lp_wave_kth(all, top));
-    if (strip.m >= least)
-      lp_walk(sp, [&](float x, int j) {
+    int reach;
+    const float least = lp_least(lp_wave_kth<false>(all, top, reach));
+    // else the list would be long or overflow: 2048 x 131072 of one value with the twenty best 109 us, listed first 268; one
+    // row of 131072 with four values and the eight best 12 us, listed first 93
+    const bool ties = reach > 2 * top + 16;
+    if (!ties) {
+      lp_walk_some(sp, strip.m >= least, sh, [&](float x, int j) {
         if (x >= least) {
           const int at = atomicAdd(&sh.listed, 1);
           if (at < LP_LIST) sh.list[at] = lp_key(x, j0 + (uint32_t)j);
         }
       });
-    __syncthreads();
-    listed = sh.listed;
+      listed = sh.listed;
+    }
+    if (ties || listed > LP_LIST) listed = lp_block_ties(sp, j0, top, lp_order(strip.m), lp_wave_kth<true>(all, top, reach), sh);
   }
   if (listed <= LP_LIST) {
     lp_rank_list(sh.list, listed, top, out);
@@ -441,7 +593,7 @@ __device__ __forceinline__ void lp_block_top(const LpSpan<T>& sp, uint32_t j0, i
   uint64_t below = ~0ull, best = 0;
   auto search = [&]() {
     best = 0;
-    lp_walk(sp, [&](float x, int j) {
+    lp_walk<LP_THREADS>(sp, threadIdx.x, [&](float x, int j) {
       const uint64_t k = lp_key(x, j0 + (uint32_t)j);
       if (k < below && k > best) best = k;
     });

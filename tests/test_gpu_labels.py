@@ -346,3 +346,48 @@ def test_refusals_on_the_device(gpu_device):
         leaf.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         got.log_prob.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K", [300, 1000, 2047, 2048, 2049, 5003, 40001, 131072])
+def test_top_where_many_are_equal(gpu_device, K, dtype):
+    """Rows of mostly one value, in the places where it matters: what is above it anywhere, equal ones only at the end of
+    the row or around one place, few or many above them in one thread's reach; few rows (in segments) and many."""
+    from gsplat.losses import label_log_probs
+
+    g = torch.Generator().manual_seed(K)
+    rows = []
+    for tie in (0.3, -0.3, -INF, 0.0):
+        low = -INF if tie == -INF else tie - 1.0
+        base = torch.full((K,), tie)
+        rows.append(base)
+        x = base.clone()  # three above
+        x[torch.randint(0, K, (3,), generator=g)] = torch.tensor([1.0, 2.0, 1.0])
+        rows.append(x)
+        x = torch.full((K,), low)  # equal ones at the end
+        x[-70:] = tie
+        x[0], x[K // 2] = tie, 3.0
+        rows.append(x)
+        x = torch.where(torch.rand(K, generator=g) < 0.1, torch.tensor(tie), torch.tensor(low))
+        rows.append(x)
+        for every, count in ((256 * 4, 9), (256 * 8, 9), (64 * 4, 3), (64 * 8, 40)):  # the places of some threads' vectors
+            x = base.clone()
+            j = torch.arange(K)
+            near = j % every < count * 4
+            x[near] = torch.randint(1, 9, (int(near.sum()),), generator=g).float()
+            rows.append(x)
+        x = base.clone()  # more above them than any list takes
+        x[::3] = torch.randint(1, 200, (len(x[::3]),), generator=g).float()
+        rows.append(x)
+    x = torch.stack(rows).to(dtype)
+    for shift in (0, 1, 3):
+        big = torch.zeros(len(rows), K + shift, dtype=dtype)
+        big[:, shift:] = x
+        xx = big.to(gpu_device)[:, shift:]
+        y = torch.zeros(len(rows), dtype=torch.long, device=gpu_device)
+        for top in (1, 5, 20, 33, 64):
+            want = x.float().sort(dim=1, descending=True, stable=True).indices[:, :top]
+            print(f"equal {dtype} {K} shift {shift} top {top}", flush=True)
+            assert torch.equal(label_log_probs(xx, y, top_k=top).top_labels.cpu(), want)
+            many = label_log_probs(xx.repeat(1100 // len(rows) + 1, 1) if shift == 0 else xx, y.repeat(1100 // len(rows) + 1) if shift == 0 else y, top_k=top)
+            assert torch.equal(many.top_labels[-len(rows):].cpu(), want)
