@@ -12,6 +12,8 @@
 #include <torch/csrc/autograd/graph_task.h>
 #include <torch/extension.h>
 
+#include <unordered_set>
+
 #include "../../include/gsplat_mi355x.h"
 
 namespace {
@@ -88,8 +90,8 @@ struct Launch {
 
 Tensor bytes(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kByte)); }
 
-// dense rows with their elements next to each other
-Tensor rows_of(const Tensor& t) { return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous(); }
+// dense rows with their elements next to each other, in memory as they are (a lazily negated view is not)
+Tensor rows_of(const Tensor& t) { return (t.size(1) <= 1 || t.stride(1) == 1) && !t.is_neg() ? t : t.resolve_neg().contiguous(); }
 
 // A gradient that nothing can be differentiated through again: a second backward reaches an error, not a zero.
 Tensor once(const Tensor& v, const char* what) {
@@ -97,25 +99,37 @@ Tensor once(const Tensor& v, const char* what) {
   return (*fail)({v.detach().requires_grad_(true)})[0];
 }
 
-// Called by a backward before it launches anything.  While a graph captures the backward, a leaf whose gradient would be
-// accumulated on another stream (an eager graph of that leaf, still alive, has made the node that does it) would pull that
-// stream into the capture, which ends the process: an error instead.
+// Called by a backward before it launches anything.  While a graph captures the backward, a leaf further down whose gradient
+// would be accumulated on another stream (an eager graph of that leaf, still alive, has made the node that does it) would
+// pull that stream into the capture, which ends the process: an error instead.  Where the gradient is only handed out, the
+// engine still makes the node's stream wait, which the default stream must not do during a capture.
 void check_capture(const Tensor& grad) {
-  const auto node = torch::autograd::get_current_node();
-  if (!node) return;
-  for (const auto& edge : node->next_edges()) {
-    auto* leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get());
-    if (!leaf) continue;
-    const auto there = leaf->stream();
-    if (!there || *there == c10::impl::VirtualGuardImpl(grad.device().type()).getStream(grad.device())) continue;
-    const auto* tasks = torch::autograd::get_current_graph_task_exec_info();
-    if (tasks && !tasks->empty()) {  // torch.autograd.grad: nothing is accumulated
-      const auto it = tasks->find(leaf);
-      if (it == tasks->end() || !it->second.needed_) continue;
+  const auto current = torch::autograd::get_current_node();
+  auto* const node = current.get();
+  if (!node || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const c10::impl::VirtualGuardImpl streams(grad.device().type());
+  const auto here = streams.getStream(grad.device()), unnamed = streams.getDefaultStream(grad.device());
+  const auto* tasks = torch::autograd::get_current_graph_task_exec_info();  // of torch.autograd.grad: what it needs
+  std::unordered_set<torch::autograd::Node*> seen{node};
+  std::vector<torch::autograd::Node*> left{node};
+  while (!left.empty()) {
+    auto* const at = left.back();
+    left.pop_back();
+    for (const auto& edge : at->next_edges()) {
+      auto* const next = edge.function.get();
+      if (!next || !seen.insert(next).second) continue;
+      if (tasks && !tasks->empty()) {
+        const auto it = tasks->find(next);
+        if (it == tasks->end() || !it->second.should_execute()) continue;
+      }
+      left.push_back(next);
+      if (!dynamic_cast<torch::autograd::AccumulateGrad*>(next)) continue;
+      const bool kept = !tasks || tasks->empty() || tasks->at(next).needed_;  // else it is handed out, not accumulated
+      const auto there = next->stream();
+      TORCH_CHECK(!there || *there == here || (!kept && *there != unnamed),
+                  "gsplat (MI355X build): this backward is being captured while an eager graph of the same leaf, made on "
+                  "another stream, is alive: delete its outputs before the capture");
     }
-    TORCH_CHECK(c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
-                "gsplat (MI355X build): this backward is being captured while an eager graph of the same leaf, made on "
-                "another stream, is alive: delete its outputs before the capture");
   }
 }
 
@@ -229,7 +243,7 @@ std::vector<Tensor> checked(const std::vector<Tensor>& grads) {
     dtype_code(g);
     require_gpu(g, grads[0]);
     // values that fill their memory, in whatever order of dimensions, are taken as they lie
-    raw.push_back(g.is_non_overlapping_and_dense() ? g : g.contiguous());
+    raw.push_back(g.is_non_overlapping_and_dense() && !g.is_neg() ? g : g.resolve_neg().contiguous());
   }
   return raw;
 }

@@ -339,3 +339,66 @@ def test_captured_backward_next_to_an_eager_graph_is_refused(gpu_device):
         assert bool(torch.isfinite(table.grad).all())
         table.grad = None
         del eager, graph
+
+
+def test_captured_backward_behind_other_nodes_is_refused_too(gpu_device):
+    """The leaf lies behind views and products here, or its gradient is asked for and not accumulated: an eager graph made
+    on a stream of its own is in nobody's way then."""
+    from gsplat.losses import label_log_probs
+    from gsplat.prepass import embedding_lookup
+
+    dev = gpu_device
+    table = torch.randn(2, 10, 8, device=dev).requires_grad_(True)
+    ids, labels = torch.arange(20, device=dev), torch.arange(20, device=dev).view(2, 10) % 8
+    for make in (lambda: embedding_lookup((table * 2.0).view(20, 8), ids).sum(), lambda: label_log_probs(table, labels).log_prob.sum()):
+        make().backward()  # (warm)
+        want, table.grad = table.grad, None
+        eager = make()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="eager graph of the same leaf"):
+            with torch.cuda.graph(graph):
+                make().backward()
+        eager.backward()
+        assert torch.equal(table.grad, want)
+        table.grad = None
+        eager = make()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="eager graph of the same leaf"):
+            with torch.cuda.graph(graph):
+                torch.autograd.grad(make(), table)
+        del eager
+        side = torch.cuda.Stream(dev)
+        side.wait_stream(torch.cuda.current_stream(dev))
+        with torch.cuda.stream(side):
+            eager = make()
+        torch.cuda.current_stream(dev).wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got, = torch.autograd.grad(make(), table)
+        for _ in range(3):
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+        del eager, graph, got
+
+
+def test_negated_views(gpu_device):
+    """Tensors that torch negates lazily hold the other sign in memory."""
+    from gsplat.gradients import clip_gradients
+    from gsplat.losses import label_log_probs
+    from gsplat.prepass import embedding_lookup
+
+    dev = gpu_device
+    x = torch.randn(30, 9, device=dev)
+    neg = torch.complex(torch.zeros_like(x), x).conj().imag
+    assert neg.is_neg() and torch.equal(neg, -x)
+    plain = (-x).contiguous()
+    ids, labels = torch.arange(20, device=dev) % 30, torch.arange(30, device=dev) % 9
+    assert torch.equal(embedding_lookup(neg, ids), embedding_lookup(plain, ids))
+    assert all(torch.equal(a, b) for a, b in zip(label_log_probs(neg, labels, 3), label_log_probs(plain, labels, 3)))
+    (a,), norm_a = clip_gradients([neg], 0.5)
+    (b,), norm_b = clip_gradients([plain], 0.5)
+    assert torch.equal(a, b) and torch.equal(norm_a, norm_b)
+    clip_gradients([neg], 0.5, inplace=True)
+    assert torch.equal(neg, b)
