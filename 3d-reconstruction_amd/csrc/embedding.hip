@@ -143,15 +143,26 @@ __device__ __forceinline__ uint32_t emb_key(const void* ids, int id_bytes, int64
   return id >= 0 && id < V ? (uint32_t)id : (uint32_t)V;  // ids that select nothing sort behind all rows
 }
 
-// the lanes (of those that take part) with this lane's digit of `bits` bits
-__device__ __forceinline__ unsigned long long emb_peers(uint32_t d, int bits, bool valid) {
-  unsigned long long peers = __ballot(valid);
-  for (int b = 0; b < bits; ++b) {
-    const bool bit = (d >> b) & 1u;
-    const unsigned long long m = __ballot(bit);
-    peers &= bit ? m : ~m;
+// For each of a wave's items the lanes whose item has the same digit (of `bits` bits from `shift` on), lower and upper half.
+// All items at once: ballots of one do not wait for those of another.
+template <int ITEMS>
+__device__ __forceinline__ void emb_peers(const uint32_t (&key)[ITEMS], int64_t wave_first, int64_t n, int shift, int bits,
+                                          uint32_t (&lo)[ITEMS], uint32_t (&hi)[ITEMS]) {
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const unsigned long long valid = __ballot(wave_first + i * 64 + (threadIdx.x & 63) < n);
+    lo[i] = (uint32_t)valid;
+    hi[i] = (uint32_t)(valid >> 32);
   }
-  return peers;
+  for (int b = shift; b < shift + bits; ++b) {
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+      const uint32_t bit = (uint32_t)__builtin_amdgcn_sbfe((int)key[i], b, 1);  // all ones or none
+      const unsigned long long m = __ballot(bit != 0);
+      lo[i] &= ~((uint32_t)m ^ bit);
+      hi[i] &= ~((uint32_t)(m >> 32) ^ bit);
+    }
+  }
 }
 
 // One digit of the items that a workgroup holds in registers, wave by wave in their order: cnt [waves][radix] gets each
@@ -159,17 +170,17 @@ __device__ __forceinline__ unsigned long long emb_peers(uint32_t d, int bits, bo
 template <int ITEMS>
 __device__ __forceinline__ void emb_rank(const uint32_t (&key)[ITEMS], int64_t wave_first, int64_t n, int shift, int bits,
                                          uint32_t* __restrict__ cnt, uint32_t (&rank)[ITEMS]) {
-  const int lane = threadIdx.x & 63;
+  uint32_t lo[ITEMS], hi[ITEMS];
+  emb_peers(key, wave_first, n, shift, bits, lo, hi);
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) {
-    const bool valid = wave_first + i * 64 + lane < n;
+    const bool valid = wave_first + i * 64 + (threadIdx.x & 63) < n;
     const uint32_t d = (key[i] >> shift) & ((1u << bits) - 1u);
-    const unsigned long long peers = emb_peers(d, bits, valid);
-    const uint32_t before = (uint32_t)__popcll(peers & ((1ull << lane) - 1ull));
+    const uint32_t before = __builtin_amdgcn_mbcnt_hi(hi[i], __builtin_amdgcn_mbcnt_lo(lo[i], 0));
     const uint32_t prev = cnt[d];
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    if (valid && before == 0) cnt[d] = prev + (uint32_t)__popcll(peers);
+    if (valid && before == 0) cnt[d] = prev + (uint32_t)(__popc(lo[i]) + __popc(hi[i]));
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     rank[i] = prev + before;
@@ -195,8 +206,8 @@ template <int THREADS> __device__ __forceinline__ uint32_t emb_scan(uint32_t v, 
   return before + incl - v;
 }
 
-// Workgroup 0 sorts up to 1024 ITEMS ids in LDS, digits of at most 8 bits; the others fill.  16384 ids of 13 bits take 34 us
-// (a chain of ballots and LDS words in one CU), which the zeros of a 268 MB table hide: 50 us together, 5.4 TB/s of stores.
+// Workgroup 0 sorts up to 1024 ITEMS ids in LDS, digits of at most 8 bits; the others fill.  16384 ids of 13 bits take 22 us
+// (ballots and LDS words in one CU), 3000 8 us; the zeros of a 268 MB table hide it: 50 us together, 5.4 TB/s of stores.
 template <int ITEMS>
 __global__ __launch_bounds__(EMB_SORT1_THREADS) void embed_sort1_kernel(int n, int64_t V, int bits,
                                                                         const void* __restrict__ ids, int id_bytes,
@@ -242,29 +253,31 @@ __global__ __launch_bounds__(EMB_SORT1_THREADS) void embed_sort1_kernel(int n, i
     for (int i = 0; i < ITEMS; ++i)
       if (first + i * 64 + lane < n) {
         const uint32_t to = cnt[wave][(key[i] >> shift) & ((1u << width) - 1u)] + rank[i];
-        if (p == passes - 1) {
-          keys_out[to] = key[i];
-          pos_out[to] = pos[i];
-        } else {
-          keys[to] = key[i];
-          poss[to] = pos[i];
-        }
+        keys[to] = key[i];
+        poss[to] = pos[i];
       }
     __syncthreads();
-    if (p < passes - 1) {
 #pragma unroll
-      for (int i = 0; i < ITEMS; ++i) {
-        const int at = first + i * 64 + lane;
-        key[i] = at < n ? keys[at] : 0;
-        pos[i] = at < n ? poss[at] : 0;
-      }
+    for (int i = 0; i < ITEMS; ++i) {
+      const int at = first + i * 64 + lane;
+      key[i] = at < n ? keys[at] : 0;
+      pos[i] = at < n ? poss[at] : 0;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {  // (out of LDS too: words scattered over the lists would go out one a cycle)
+    const int at = first + i * 64 + lane;
+    if (at < n) {
+      keys_out[at] = key[i];
+      pos_out[at] = pos[i];
     }
   }
 }
 
 // One digit of the radix sort: the digits' counts per workgroup (digit by digit), their sums over the workgroups before,
 // and the scatter.  `keys` NULL: the first digit, straight from the ids.  Workgroups from `blocks` on fill.  1M ids of 7
-// bits: 9 + 6 + 16 us; bound by latency and, in the scatter, by stores of single words.
+// bits: 7 + 4 + 10 us, a digit of 9 bits 9 + 4 + 14; bound by latency.  The scatter goes through LDS, where a workgroup's
+// items of a digit come to lie next to each other (9 bits straight from registers: 24 us; 4096 items a workgroup: 18 us).
 struct EmbDigit {
   int64_t n, V;
   const void* ids;
@@ -296,13 +309,12 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_hist_kernel(EmbDigit s) {
   const int64_t first = (int64_t)blockIdx.x * EMB_TILE + (threadIdx.x >> 6) * (64 * EMB_ITEMS);
   uint32_t key[EMB_ITEMS];
   emb_load_items(s, first, key);
+  uint32_t lo[EMB_ITEMS], hi[EMB_ITEMS];
+  emb_peers(key, first, s.n, s.shift, s.bits, lo, hi);
 #pragma unroll
-  for (int i = 0; i < EMB_ITEMS; ++i) {  // one addition per digit that a wave holds: grouped ids would queue up
-    const bool valid = first + i * 64 + lane < s.n;
-    const uint32_t d = (key[i] >> s.shift) & ((1u << s.bits) - 1u);
-    const unsigned long long peers = emb_peers(d, s.bits, valid);
-    if (valid && (peers & ((1ull << lane) - 1ull)) == 0) atomicAdd(&hist[d], (uint32_t)__popcll(peers));
-  }
+  for (int i = 0; i < EMB_ITEMS; ++i)  // one addition per digit that a wave holds: grouped ids would queue up
+    if (first + i * 64 + lane < s.n && __builtin_amdgcn_mbcnt_hi(hi[i], __builtin_amdgcn_mbcnt_lo(lo[i], 0)) == 0)
+      atomicAdd(&hist[(key[i] >> s.shift) & ((1u << s.bits) - 1u)], (uint32_t)(__popc(lo[i]) + __popc(hi[i])));
   __syncthreads();
   for (int d = threadIdx.x; d < 1 << s.bits; d += EMB_THREADS) s.table[(int64_t)d * s.blocks + blockIdx.x] = hist[d];
 }
@@ -316,18 +328,28 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_digit_sums_kernel(EmbDigit 
   }
   const int lane = threadIdx.x & 63, d = blockIdx.x * (EMB_THREADS / 64) + (threadIdx.x >> 6);
   if (d >= 1 << s.bits) return;
+  constexpr int PER = 8;
   uint32_t* row = s.table + (int64_t)d * s.blocks;
   uint32_t run = 0;
-  for (int c0 = 0; c0 < s.blocks; c0 += 64) {
-    const int c = c0 + lane;
-    const uint32_t v = c < s.blocks ? row[c] : 0u;
-    uint32_t incl = v;
+  for (int c0 = 0; c0 < s.blocks; c0 += 64 * PER) {  // PER in succession to a lane: one scan for all of them
+    const int c = c0 + lane * PER;
+    uint32_t v[PER], sum = 0;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) v[k] = c + k < s.blocks ? row[c + k] : 0u;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) sum += v[k];
+    uint32_t incl = sum;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const uint32_t t = __shfl_up(incl, o);
       if (lane >= o) incl += t;
     }
-    if (c < s.blocks) row[c] = run + incl - v;
+    uint32_t before = run + incl - sum;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      if (c + k < s.blocks) row[c + k] = before;
+      before += v[k];
+    }
     run += __shfl(incl, 63);
   }
   if (lane == 0) s.totals[d] = run;
@@ -341,6 +363,7 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_scatter_kernel(EmbDigit s) 
   constexpr int WAVES = EMB_THREADS / 64, PER = EMB_RADIX / EMB_THREADS;
   __shared__ uint32_t cnt[WAVES][EMB_RADIX];
   __shared__ uint32_t start[EMB_RADIX];
+  __shared__ uint32_t keys[EMB_TILE], poss[EMB_TILE];
   __shared__ uint32_t wsum[WAVES];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, radix = 1 << s.bits;
   const int64_t first = (int64_t)blockIdx.x * EMB_TILE + wave * (64 * EMB_ITEMS);
@@ -366,13 +389,24 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_scatter_kernel(EmbDigit s) 
   }
   emb_rank<EMB_ITEMS>(key, first, s.n, s.shift, s.bits, cnt[wave], rank);
   __syncthreads();
-  for (int d = threadIdx.x; d < radix; d += EMB_THREADS) {
-    uint32_t at = start[d] + s.table[(int64_t)d * s.blocks + blockIdx.x];
+  sum = 0;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    t[k] = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) t[k] += cnt[w][threadIdx.x * PER + k];
+    sum += t[k];
+  }
+  run = emb_scan<EMB_THREADS>(sum, wsum);
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    const int d = threadIdx.x * PER + k;
+    if (d < radix) start[d] += s.table[(int64_t)d * s.blocks + blockIdx.x] - run;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
       const uint32_t c = cnt[w][d];
-      cnt[w][d] = at;
-      at += c;
+      cnt[w][d] = run;
+      run += c;
     }
   }
   __syncthreads();
@@ -380,9 +414,21 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_scatter_kernel(EmbDigit s) 
   for (int i = 0; i < EMB_ITEMS; ++i)
     if (first + i * 64 + lane < s.n) {
       const uint32_t to = cnt[wave][(key[i] >> s.shift) & (uint32_t)(radix - 1)] + rank[i];
-      s.keys_out[to] = key[i];
-      s.pos_out[to] = pos[i];
+      keys[to] = key[i];
+      poss[to] = pos[i];
     }
+  __syncthreads();
+  const int64_t base = (int64_t)blockIdx.x * EMB_TILE;
+  const int n = (int)(s.n - base < EMB_TILE ? s.n - base : EMB_TILE);
+#pragma unroll
+  for (int i = 0; i < EMB_ITEMS; ++i) {
+    const int at = i * EMB_THREADS + threadIdx.x;
+    if (at < n) {
+      const uint32_t k = keys[at], to = start[(k >> s.shift) & (uint32_t)(radix - 1)] + at;
+      s.keys_out[to] = k;
+      s.pos_out[to] = poss[at];
+    }
+  }
 }
 
 // ---- sums of the runs
@@ -569,7 +615,7 @@ __global__ __launch_bounds__(EMB_JOIN_THREADS) void embed_join_kernel(EmbShape s
 // ---- few rows (V <= EMB_FEW, of D <= 128 columns): no sort.  256 threads read 256 values at a time, several rows, a column
 // each, and add them to a table in LDS that belongs to the thread's place among those rows: no two threads meet in a word.
 // Equal ids in succession, the rule where Gaussians lie instance by instance, add up in a register first.  The tables of a workgroup are added up, in their order, and embed_few_join_kernel adds the workgroups'.
-// 1M x 16 fp32 on 64 rows: 24 + 4 us (3.0 TB/s; LDS leaves a CU eight waves), against 64 us by the sort.
+// 1M x 16 fp32 on 64 rows: 24 + 4 us (3.0 TB/s; LDS leaves a CU eight waves), against 55 us by the sort.
 struct EmbFew {
   int64_t n, per, gs;   // ids, ids of a workgroup, row stride of v_out
   int32_t V, D, Dp;     // Dp: D rounded up to a power of two
@@ -736,8 +782,8 @@ static int emb_bits(int64_t V) {
 
 static int64_t emb_round(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 
-// Tables beyond the Infinity Cache are better zeroed in one sweep: 64 ids on 131072 x 512 fp32 take 37 us directly and 45 us
-// sorted, on 131072 x 1024 141 and 119 us.
+// Tables beyond the Infinity Cache are better zeroed in one sweep: 64 ids on 131072 x 512 fp32 take 37 us directly and 41 us
+// sorted, on 131072 x 1024 141 and 116 us.
 static bool emb_direct(int64_t n, int64_t V, int64_t D) { return n <= EMB_DIRECT && V * D <= (int64_t)1 << 26; }
 
 struct EmbWorkspace {
@@ -756,8 +802,8 @@ static int emb_piece(int64_t n, int64_t D) {
 static int emb_longest(int64_t n, int64_t D) { return n >= 131072 ? EMB_LONG_MAX : std::max(16, emb_piece(n, D)); }
 
 // The form for few rows is taken where a workgroup reads two rows or more at a time: gradients alone, by it and by the sort,
-// 1M ids on 64 x 16 fp32 31 and 67 us, 38358 on 6 x 36 10 and 29, 20000 on 64 x 64 17 and 35, 300 on 64 x 64 16 and 16; but
-// 100000 on 64 x 256 55 and 48, on 64 x 1024 143 and 74.
+// 1M ids on 64 x 16 fp32 32 and 59 us, 38358 on 6 x 36 10 and 28, 20000 on 64 x 64 17 and 31, 300 on 64 x 64 16 and 13; but
+// 100000 on 64 x 256 55 and 46, on 64 x 1024 143 and 72.
 static bool emb_few(int64_t V, int64_t D) { return V <= EMB_FEW && D <= EMB_THREADS / 2; }
 
 // Its workgroups: two on each CU, each with twice as many ids as the table has rows or more, so that writing and adding up
