@@ -100,8 +100,9 @@ struct EmbShape {
   float scale;
 };
 
-// The sorted sums go past the caches: the rows of v_out that are still to be read stay there instead.  200003 ids on
-// 32000 x 512 bf16, lookup and gradient: 176 -> 146 us, 187 -> 158 us with a pass over the gradient behind it.
+// The sorted sums go past the caches: the rows of v_out that are still to be read stay there instead.  Lookup and gradient,
+// plain and past the caches: 100000 ids on 50000 x 256 fp32 101 and 97 us, 16384 on 131072 x 1024 bf16 81 and 79, 200003 on
+// 32000 x 512 bf16 174 and 174 (185 and 191 with a pass over the gradient behind it).
 template <typename T, int N, bool NT = true>
 __device__ __forceinline__ void emb_store(T* __restrict__ p, const float (&acc)[N], float scale) {
   float x[N];
@@ -112,8 +113,8 @@ __device__ __forceinline__ void emb_store(T* __restrict__ p, const float (&acc)[
 
 // ---- the table's zeros, in `shares` stretches of whole vectors (the first also has what lies before and behind them)
 // With ids for an eighth of the rows and more they go past the caches, for the same reason as the sums; with fewer the
-// plain stores are faster.  131072 x 1024 bf16, lookup and gradient, plain / past the caches: 4096 ids 64 / 73 us, 8192
-// ids 77 / 76 us, 16384 ids 93 / 84 us, 65536 ids 193 / 177 us.
+// plain stores are faster.  131072 x 1024 bf16, lookup and gradient, plain / past the caches: 4096 ids 63 / 73 us, 8192
+// ids 73 / 74 us, 16384 ids 87 / 79 us, 65536 ids 190 / 180 us.
 struct EmbFill {
   char* base;
   int64_t bytes;
@@ -441,9 +442,26 @@ __device__ __forceinline__ int64_t emb_lower(const uint32_t* keys, int64_t lo, i
   return lo;
 }
 
+// adds up the groups' sums, in their order, in group 0; lds [N][THREADS]
+template <int THREADS, int N>
+__device__ __forceinline__ void emb_add_groups(float (&acc)[N], int g, int G, float* __restrict__ lds) {
+  for (int half = THREADS / G / 2; half > 0; half /= 2) {
+    if (g >= half && g < 2 * half)
+#pragma unroll
+      for (int k = 0; k < N; ++k) lds[k * THREADS + threadIdx.x] = acc[k];
+    __syncthreads();
+    if (g < half)
+#pragma unroll
+      for (int k = 0; k < N; ++k) acc[k] += lds[k * THREADS + half * G + threadIdx.x];
+    __syncthreads();
+  }
+}
+
 // A group of G lanes takes the P sorted entries [i0, i1); its workgroup has their keys in LDS, with `longest` more on both
 // sides.  partial [pieces][2][D] fp32: what lies in the piece of the long run that started before it (slot 0), and of the
-// long run that starts in it (slot 1; there is one at most, and it goes on behind the piece).  Bound by the latency of
+// long run that starts in it (slot 1; there is one at most, and it goes on behind the piece).  A workgroup that has nothing
+// but entries of a run that started before it adds up all its pieces, in slot 0 of the first, and has zeros for the others.
+// Bound by the latency of
 // scattered rows, FLIGHT of them a group: 1M rows of 64 bytes 24 us in 65 runs and 31 us in 200000 (2.7 and 2.5 TB/s),
 // 16384 rows of 2 KB 14 us (3.8 TB/s with the stored sums).
 template <typename T, int N>
@@ -468,9 +486,36 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_runs_kernel(EmbShape sh, co
   const uint32_t* key = lkey + M + g * P;  // key[0]: the piece's first entry
   const uint32_t* at = lpos + g * P;
   const int64_t i0 = w0 + (int64_t)g * P;
+  const uint32_t V = (uint32_t)sh.V, one = lkey[M];
+  if (w0 + span <= sh.n && lkey[M - 1] == one && lkey[M + span - 1] == one && one < V) {  // (span >= longest: a long run)
+    float acc[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) acc[k] = 0.f;
+    if (vec < sh.vpr)
+      for (int i = 0; i < P; i += FLIGHT) {
+        Raw<T, N> raw[FLIGHT];
+#pragma unroll
+        for (int u = 0; u < FLIGHT; ++u) raw[u] = load_raw<T, N>(v_out + (int64_t)at[i + u < P ? i + u : P - 1] * sh.gs + vec * N);
+#pragma unroll
+        for (int u = 0; u < FLIGHT; ++u)
+          if (i + u < P) {
+            float x[N];
+            unpack<T, N>(raw[u], x);
+#pragma unroll
+            for (int k = 0; k < N; ++k) acc[k] += x[k];
+          }
+      }
+    __syncthreads();  // the keys and positions have been read
+    emb_add_groups<EMB_THREADS, N>(acc, g, sh.G, (float*)lds);
+    if (vec < sh.vpr) {
+      float* to = partial + 2 * (i0 / P) * (sh.vpr * N) + vec * N;
+#pragma unroll
+      for (int k = 0; k < N; ++k) to[k] = g == 0 ? acc[k] : 0.f;
+    }
+    return;
+  }
   if (i0 >= sh.n || vec >= sh.vpr) return;
   const int i1 = sh.n - i0 < P ? (int)(sh.n - i0) : P;
-  const uint32_t V = (uint32_t)sh.V;
 
   int a = 0;            // first entry to add
   bool before = false;  // ... which belongs to a long run that started before the piece
@@ -523,22 +568,20 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_runs_kernel(EmbShape sh, co
   }
 }
 
-// Adds the partial sums of the pieces first, first + step, ... of the long run of `key` that starts in piece `start`.  A
-// piece is the run's exactly where its first entry is.  EMB_JOIN_FLIGHT are read at a time, whether they are or not: asking
-// first would cost a trip to memory for each.
+// Adds the partial sums of the long run of `key` that starts in piece `start`.  A piece is the run's exactly where its first
+// entry is.  EMB_JOIN_FLIGHT are read at a time, whether they are or not: asking first would cost a trip to memory for each.
 template <int N>
-__device__ __forceinline__ void emb_add_pieces(float (&acc)[N], const uint32_t* __restrict__ keys, int64_t pieces, int P,
-                                               uint32_t key, int64_t start, int64_t first, int64_t step,
-                                               const float* __restrict__ partial, int64_t D, int64_t col) {
+__device__ __forceinline__ void emb_add_pieces(float (&acc)[N], const uint32_t* __restrict__ keys, int pieces, int P,
+                                               uint32_t key, int start, const float* __restrict__ partial, int64_t D) {
   bool more = true;
-  for (int64_t r = first; more; r += EMB_JOIN_FLIGHT * step) {
+  for (int r = start; more; r += EMB_JOIN_FLIGHT) {
     float x[EMB_JOIN_FLIGHT][N];
     bool in[EMB_JOIN_FLIGHT];
 #pragma unroll
     for (int u = 0; u < EMB_JOIN_FLIGHT; ++u) {
-      const int64_t c = r + u * step, d = c < pieces ? c : pieces - 1;
+      const int c = r + u, d = c < pieces ? c : pieces - 1;
       in[u] = c == start || (c < pieces && keys[d * P] == key);
-      const float* src = partial + (2 * d + (c == start ? 1 : 0)) * D + col;
+      const float* src = partial + (2 * d + (c == start ? 1 : 0)) * D;
 #pragma unroll
       for (int k = 0; k < N; ++k) x[u][k] = src[k];
     }
@@ -551,16 +594,20 @@ __device__ __forceinline__ void emb_add_pieces(float (&acc)[N], const uint32_t* 
 }
 
 // A workgroup looks at some pieces for long runs that start in them.  One of its groups takes a run of few pieces; all take
-// one of many, and are joined in LDS, in their order.  5 us where there are none of 1M ids, 10 us for 65 of 15000, 120 us
-// for one of all of them, which one workgroup adds up.
+// one of many: its pieces up to the first stretch of `per` pieces that a workgroup of embed_runs_kernel added up, the sums
+// of those stretches, and the pieces behind the last; the groups are added up in LDS, in their order.  4 us where there are
+// none of 1M ids, 9 us for 65 of 15000, 10 us for one of all of them (120 us by its pieces alone).
 template <typename T, int N>
 __global__ __launch_bounds__(EMB_JOIN_THREADS) void embed_join_kernel(EmbShape sh, const uint32_t* __restrict__ keys,
                                                                       const float* __restrict__ partial,
                                                                       T* __restrict__ v_table) {
   __shared__ float lds[EMB_JOIN_THREADS * N];
   __shared__ int found[2][EMB_JOIN_PIECES], count[2];  // [longer ones]: pieces in which such a run starts
+  __shared__ int behind;  // stretch in which the run ends
+  constexpr int FLIGHT = EMB_JOIN_FLIGHT / 2;  // stretches
   const int P = sh.piece;
   const int g = threadIdx.x / sh.G, groups = EMB_JOIN_THREADS / sh.G, few = groups / 2 > 32 ? groups / 2 : 32;
+  const int per = EMB_THREADS / sh.G;  // pieces of a workgroup of embed_runs_kernel; `few` are two of them or more
   const int64_t p0 = (int64_t)blockIdx.x * sh.join, pieces = (sh.n + P - 1) / P;
   if (threadIdx.x < 2) count[threadIdx.x] = 0;
   __syncthreads();
@@ -588,7 +635,7 @@ __global__ __launch_bounds__(EMB_JOIN_THREADS) void embed_join_kernel(EmbShape s
       float acc[N];
 #pragma unroll
       for (int k = 0; k < N; ++k) acc[k] = 0.f;
-      emb_add_pieces<N>(acc, keys, pieces, P, key, p, p, 1, partial, D, col);
+      emb_add_pieces<N>(acc, keys, (int)pieces, P, key, (int)p, partial + col, D);
       emb_store<T, N>(v_table + (int64_t)key * D + col, acc, sh.scale);
     }
   for (int q = 0; q < count[1]; ++q) {
@@ -597,17 +644,53 @@ __global__ __launch_bounds__(EMB_JOIN_THREADS) void embed_join_kernel(EmbShape s
     float acc[N];
 #pragma unroll
     for (int k = 0; k < N; ++k) acc[k] = 0.f;
-    if (vec < sh.vpr) emb_add_pieces<N>(acc, keys, pieces, P, key, p, p + g, groups, partial, D, col);
-    for (int half = groups / 2; half > 0; half /= 2) {
-      if (g >= half && g < 2 * half)
+    auto add = [&](const float* src) {
 #pragma unroll
-        for (int k = 0; k < N; ++k) lds[k * EMB_JOIN_THREADS + threadIdx.x] = acc[k];
-      __syncthreads();
-      if (g < half)
+      for (int k = 0; k < N; ++k) acc[k] += src[k];
+    };
+    const int n = (int)sh.n, s0 = (int)p / per + 1;  // first stretch behind the one where it starts
+    const float* sums = partial + (vec < sh.vpr ? col : 0);
+    if (threadIdx.x == 0) behind = 0x7fffffff;
+    __syncthreads();
+    if ((int)p + g < s0 * per) add(sums + (2 * (p + g) + (g == 0 ? 1 : 0)) * D);  // (all are the run's)
+    bool more = true;
+    int end_at = 0x7fffffff;
+    for (int r = s0 + g; more; r += FLIGHT * groups) {
+      float x[FLIGHT][N];
+      bool in[FLIGHT];
 #pragma unroll
-        for (int k = 0; k < N; ++k) acc[k] += lds[k * EMB_JOIN_THREADS + half * sh.G + threadIdx.x];
-      __syncthreads();
+      for (int u = 0; u < FLIGHT; ++u) {
+        const int c = r + u * groups;
+        const uint32_t end = (uint32_t)(c + 1) * (per * P);  // (n is below 2^30, what is added to it far below that)
+        const bool there = end <= (uint32_t)n;
+        in[u] = there && keys[(there ? end : n) - 1] == key;
+        const float* src = sums + 2 * (there ? c * per : p) * D;
+#pragma unroll
+        for (int k = 0; k < N; ++k) x[u][k] = src[k];
+      }
+#pragma unroll
+      for (int u = FLIGHT - 1; u >= 0; --u)
+        if (!in[u]) end_at = r + u * groups;
+#pragma unroll
+      for (int u = 0; u < FLIGHT; ++u)
+#pragma unroll
+        for (int k = 0; k < N; ++k) acc[k] += in[u] ? x[u][k] : 0.f;
+      more = in[FLIGHT - 1];
     }
+    for (int o = 1; o < 64; o <<= 1) end_at = min(end_at, __shfl_xor(end_at, o));
+    if ((threadIdx.x & 63) == 0) atomicMin(&behind, end_at);
+    __syncthreads();
+    const int c = behind * per + g;  // the rest of them, in the stretch where the run ends
+    if (g < per && c < pieces) {
+      const float* src = sums + 2 * (int64_t)c * D;
+      float x[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) x[k] = src[k];
+      const bool in = keys[c * P] == key;
+#pragma unroll
+      for (int k = 0; k < N; ++k) acc[k] += in ? x[k] : 0.f;
+    }
+    emb_add_groups<EMB_JOIN_THREADS, N>(acc, g, sh.G, lds);
     if (g == 0 && vec < sh.vpr) emb_store<T, N>(v_table + (int64_t)key * D + col, acc, sh.scale);
   }
 }
@@ -796,10 +879,10 @@ static int emb_piece(int64_t n, int64_t D) {
   return n * D < ((int64_t)1 << 20) ? 4 : n * D < ((int64_t)1 << 26) ? 16 : EMB_LONG_MAX;
 }
 
-// With many groups a run may keep one of them busy for longer, which saves the join: 1M ids on 65 x 16 and on 200000 x 16
-// fp32 take 91 and 142 us with runs of up to 16, 64 and 113 us with 64.  With few groups that one is what all wait for:
-// 16384 ids on 131072 x 1024 bf16 take 86 and 98 us.
-static int emb_longest(int64_t n, int64_t D) { return n >= 131072 ? EMB_LONG_MAX : std::max(16, emb_piece(n, D)); }
+// Runs that one group adds up by itself: longer ones keep it busy while the others wait (16 or 64 as the longest: 16384 ids
+// of a skewed choice of 5000 x 64 fp32 43 and 49 us, 1M of 200000 x 16 120 and 124; 1M spread over 50000 x 16 80 and 77).
+// No fewer than a piece, no more than what a workgroup of embed_runs_kernel has at once.
+static int emb_longest(int64_t n, int64_t D) { return std::max(16, emb_piece(n, D)); }
 
 // The form for few rows is taken where a workgroup reads two rows or more at a time: gradients alone, by it and by the sort,
 // 1M ids on 64 x 16 fp32 32 and 59 us, 38358 on 6 x 36 10 and 28, 20000 on 64 x 64 17 and 31, 300 on 64 x 64 16 and 13; but
@@ -985,7 +1068,7 @@ extern "C" int gs_embedding_bwd(int64_t n, int64_t V, int64_t D, int32_t dtype, 
         sh.join = (int)std::min<int64_t>(std::max<int64_t>(pieces / 256, 16), EMB_JOIN_PIECES);
         const int span = EMB_THREADS / sh.G * sh.piece;
         hipLaunchKernelGGL((embed_runs_kernel<T, NV>), dim3((unsigned)ceil_div(n, span), (unsigned)tiles), dim3(EMB_THREADS),
-                           (2 * span + 3 * sh.longest + 1) * sizeof(uint32_t), s, sh, keys, pos, (const T*)v_out, partial,
+                           std::max(2 * span + 3 * sh.longest + 1, EMB_THREADS * NV) * sizeof(uint32_t), s, sh, keys, pos, (const T*)v_out, partial,
                            (T*)v_table);
         GS_CHECK_LAUNCH();
         hipLaunchKernelGGL((embed_join_kernel<T, NV>), dim3((unsigned)ceil_div(pieces, sh.join), (unsigned)tiles),

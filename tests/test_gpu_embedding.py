@@ -402,3 +402,30 @@ def test_negated_views(gpu_device):
     assert torch.equal(a, b) and torch.equal(norm_a, norm_b)
     clip_gradients([neg], 0.5, inplace=True)
     assert torch.equal(neg, b)
+
+
+@pytest.mark.parametrize("n,V,D", [(4000, 100, 16), (40_000, 100, 16), (140_000, 70, 3), (140_000, 300, 64), (20_000, 500, 260), (60_000, 90, 1200)])
+def test_runs_as_long_as_several_workgroups(gpu_device, n, V, D):
+    """Runs that start and end anywhere in what one workgroup has, from a few of its pieces to most of the ids: the sums of
+    the gradient come from single pieces, whole workgroups and both."""
+    from gsplat.prepass import embedding_lookup
+
+    dev, g = gpu_device, torch.Generator().manual_seed(n + D)
+    table, v_out = torch.zeros(V, D, device=dev).requires_grad_(True), torch.randn(n, D, generator=g)
+    up, wide, size = v_out.to(dev), v_out.double(), v_out.double().abs()
+    for lead in (0, 1, 15, 64, 257, 1024) if n * D < 10_000_000 else (0, 257):
+        for length in (16, 63, 64, 65, 256, 257, 511, 1024, 1500, 4096, n - 3000, n - lead):
+            if length < 1 or lead + length > n or (n * D > 10_000_000 and length < 256):
+                continue
+            ids = torch.full((n,), V - 1, dtype=torch.int64)
+            ids[:lead] = torch.arange(lead) % (V // 3)
+            ids[lead:lead + length] = V // 2
+            rest = n - lead - length
+            ids[lead + length:] = V // 2 + 1 + torch.arange(rest) % (V - V // 2 - 1)
+            ids = ids[torch.randperm(n, generator=g)]
+            (v,) = torch.autograd.grad(embedding_lookup(table, ids.to(dev)), table, up)
+            want, terms = torch.zeros(V, D, dtype=torch.float64), torch.zeros(V, D, dtype=torch.float64)
+            want.index_add_(0, ids, wide)
+            terms.index_add_(0, ids, size)
+            count = torch.bincount(ids, minlength=V)[:, None]
+            assert_within(f"run of {length} behind {lead} of {n}x{V}x{D}", v, want, (count + 1) * U * terms + rounding(v.dtype, want))
