@@ -408,7 +408,7 @@ __global__ __launch_bounds__(LP_THREADS, 4) void label_wave_fwd_kernel(LpFwd a, 
 // list takes what is above the k-th largest maximum and the first values that equal it.  Rows whose list overflows all the
 // same or that hold NaN take the alternatives one by one, each thread keeping its strip's best and reading the strip again
 // when it won.
-// 2048 x 100277 bf16 74 us (5.5 TB/s); one row of 131072 bf16 with its eight best 5.6 us in 64 segments and 3.4 us to join
+// 2048 x 100277 bf16 74 us (5.5 TB/s); one row of 131072 bf16 with its eight best 6.2 us in 64 segments and 3.5 us to join
 // them; 2048 x 131072 130 us with the twenty best, 109 us where all logits are equal (2.5 ms one by one).
 struct LpPart {  // of one segment
   float m, s, w, pad;
