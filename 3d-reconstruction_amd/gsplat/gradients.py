@@ -33,9 +33,10 @@ def clip_gradients(grads: Iterable[Tensor], max_norm: float, inplace: bool = Fal
                    error_if_nonfinite: bool = False) -> Tuple[List[Tensor], Tensor]:
     """Scales the gradients by `min(1, max_norm / (norm + 1e-6))`, `norm` being the one over all of them.  Returns (the
     scaled gradients, norm as a 0-d fp32 tensor): new tensors (small ones in one allocation together), or with `inplace`
-    the same ones, which are neither read a second time nor written when the norm is within `max_norm`.  A NaN norm makes every gradient NaN and an infinite one
-    makes the finite ones 0; `error_if_nonfinite` raises instead, before anything is changed (one host synchronisation and
-    one more read of the gradients).  No two gradients may share memory when they are scaled in place."""
+    the same ones, which are neither read a second time nor written when the norm is within `max_norm`.  A NaN norm makes
+    every gradient NaN and an infinite one makes the finite ones 0; `error_if_nonfinite` raises instead, before anything is
+    changed (one host synchronisation and one more read of the gradients).  No two gradients may share memory when they
+    are scaled in place."""
     grads = _listed(grads)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
