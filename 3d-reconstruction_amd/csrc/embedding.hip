@@ -33,7 +33,7 @@ constexpr int EMB_ITEMS = 8;          // ids per thread and launch of the radix 
 constexpr int EMB_TILE = EMB_THREADS * EMB_ITEMS;
 constexpr int EMB_JOIN_THREADS = 1024;
 constexpr int EMB_JOIN_PIECES = 256;  // pieces that a workgroup of the join looks at, at most
-constexpr int EMB_LONG_MAX = 64;
+constexpr int EMB_PIECE_MAX = 64;
 constexpr int EMB_FLIGHT_RUNS = 8;    // rows a group has in flight there
 constexpr int EMB_JOIN_FLIGHT = 8;    // pieces a group of the join has in flight
 
@@ -495,7 +495,8 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_runs_kernel(EmbShape sh, co
       for (int i = 0; i < P; i += FLIGHT) {
         Raw<T, N> raw[FLIGHT];
 #pragma unroll
-        for (int u = 0; u < FLIGHT; ++u) raw[u] = load_raw<T, N>(v_out + (int64_t)at[i + u < P ? i + u : P - 1] * sh.gs + vec * N);
+        for (int u = 0; u < FLIGHT; ++u)
+          raw[u] = load_raw<T, N>(v_out + (int64_t)at[i + u < P ? i + u : P - 1] * sh.gs + vec * N);
 #pragma unroll
         for (int u = 0; u < FLIGHT; ++u)
           if (i + u < P) {
@@ -697,7 +698,8 @@ __global__ __launch_bounds__(EMB_JOIN_THREADS) void embed_join_kernel(EmbShape s
 
 // ---- few rows (V <= EMB_FEW, of D <= 128 columns): no sort.  256 threads read 256 values at a time, several rows, a column
 // each, and add them to a table in LDS that belongs to the thread's place among those rows: no two threads meet in a word.
-// Equal ids in succession, the rule where Gaussians lie instance by instance, add up in a register first.  The tables of a workgroup are added up, in their order, and embed_few_join_kernel adds the workgroups'.
+// Equal ids in succession, the rule where Gaussians lie instance by instance, add up in a register first.  The tables of a
+// workgroup are added up, in their order, and embed_few_join_kernel adds the workgroups'.
 // 1M x 16 fp32 on 64 rows: 24 + 4 us (3.0 TB/s; LDS leaves a CU eight waves), against 55 us by the sort.
 struct EmbFew {
   int64_t n, per, gs;   // ids, ids of a workgroup, row stride of v_out
@@ -876,7 +878,7 @@ struct EmbWorkspace {
 // enough groups to fill the card first, then longer pieces: fewer partial sums of long runs (embed_runs_kernel with pieces of
 // 4 and of 16: 16384 ids on 5000 x 16 fp32 8.2 and 13.8 us, 1000 ids 5.7 and 9.8 us)
 static int emb_piece(int64_t n, int64_t D) {
-  return n * D < ((int64_t)1 << 20) ? 4 : n * D < ((int64_t)1 << 26) ? 16 : EMB_LONG_MAX;
+  return n * D < ((int64_t)1 << 20) ? 4 : n * D < ((int64_t)1 << 26) ? 16 : EMB_PIECE_MAX;
 }
 
 // Runs that one group adds up by itself: longer ones keep it busy while the others wait (16 or 64 as the longest: 16384 ids
@@ -1068,8 +1070,8 @@ extern "C" int gs_embedding_bwd(int64_t n, int64_t V, int64_t D, int32_t dtype, 
         sh.join = (int)std::min<int64_t>(std::max<int64_t>(pieces / 256, 16), EMB_JOIN_PIECES);
         const int span = EMB_THREADS / sh.G * sh.piece;
         hipLaunchKernelGGL((embed_runs_kernel<T, NV>), dim3((unsigned)ceil_div(n, span), (unsigned)tiles), dim3(EMB_THREADS),
-                           std::max(2 * span + 3 * sh.longest + 1, EMB_THREADS * NV) * sizeof(uint32_t), s, sh, keys, pos, (const T*)v_out, partial,
-                           (T*)v_table);
+                           std::max(2 * span + 3 * sh.longest + 1, EMB_THREADS * NV) * sizeof(uint32_t), s, sh, keys, pos,
+                           (const T*)v_out, partial, (T*)v_table);
         GS_CHECK_LAUNCH();
         hipLaunchKernelGGL((embed_join_kernel<T, NV>), dim3((unsigned)ceil_div(pieces, sh.join), (unsigned)tiles),
                            dim3(EMB_JOIN_THREADS), 0, s, sh, keys, partial, (T*)v_table);

@@ -537,7 +537,10 @@ __device__ __forceinline__ int lp_block_ties(const LpSpan<T>& sp, uint32_t j0, i
       if (w < wave) at += (int)sums[w];
       have += (int)sums[w];
     }
-    for (; bits && at < top; bits &= bits - 1) sh.list[at++] = ((uint64_t)kth << 32) | (uint32_t)~(j0 + (uint32_t)(j + __ffs((int)bits) - 1));
+    for (; bits && at < top; bits &= bits - 1) {
+      const uint32_t index = j0 + (uint32_t)(j + __ffs((int)bits) - 1);
+      sh.list[at++] = ((uint64_t)kth << 32) | (uint32_t)~index;
+    }
   };
   take(t < sp.head && lp_order((float)sp.x[t]) == kth ? 1u : 0u, t);
   for (int v0 = 0; v0 < sp.vecs && have < top; v0 += LP_THREADS) {
@@ -584,7 +587,8 @@ __device__ __forceinline__ void lp_block_top(const LpSpan<T>& sp, uint32_t j0, i
       });
       listed = sh.listed;
     }
-    if (ties || listed > LP_LIST) listed = lp_block_ties(sp, j0, top, lp_order(strip.m), lp_wave_kth<true>(all, top, reach), sh);
+    if (ties || listed > LP_LIST)
+      listed = lp_block_ties(sp, j0, top, lp_order(strip.m), lp_wave_kth<true>(all, top, reach), sh);
   }
   if (listed <= LP_LIST) {
     lp_rank_list(sh.list, listed, top, out);
