@@ -897,7 +897,7 @@ static int64_t emb_few_blocks(int64_t n, int64_t V) { return std::max<int64_t>(1
 
 static EmbWorkspace emb_workspace(int64_t n, int64_t V, int64_t D) {
   EmbWorkspace w = {};
-  if (emb_direct(n, V, D)) return w;
+  if (V == 0 || D == 0 || emb_direct(n, V, D)) return w;  // (a table without rows or columns: nothing is launched)
   if (emb_few(V, D)) {
     w.total = 4 * V * D * emb_few_blocks(n, V);
     return w;
