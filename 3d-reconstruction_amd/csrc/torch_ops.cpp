@@ -204,7 +204,7 @@ struct LabelLogProbs : torch::autograd::Function<LabelLogProbs> {
     const int64_t rows = x.size(0), K = x.size(1), top_k = top_idx.size(1);
     Tensor g[3];
     for (int i = 0; i < 3; ++i)
-      if (grads[i].defined() && (i < 2 || top_k > 0)) g[i] = grads[i].to(at::kFloat).contiguous();
+      if (grads[i].defined() && (i < 2 || top_k > 0)) g[i] = grads[i].to(at::kFloat).resolve_neg().contiguous();
     if (!g[0].defined() && !g[1].defined() && !g[2].defined()) return {Tensor(), Tensor(), Tensor()};
     Tensor v = at::empty({rows, K}, x.options());
     auto ptr = [](const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; };

@@ -2,7 +2,39 @@
 import pytest
 import torch
 
+from test_gpu_labels import _case
+
 pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------- label gradient
+@pytest.mark.parametrize("rows,K", [(1, 9), (30, 9), (7, 300), (5, 5000)])
+def test_label_gradients_that_come_lazily_negated(gpu_device, rows, K):
+    """autograd hands on gradients that hold the other sign in memory, contiguous or not."""
+    from gsplat.losses import label_log_probs
+
+    dev = gpu_device
+    x, y, g = _case(rows, K, torch.float32, rows + K)
+    ups = [torch.randn(rows, generator=g).to(dev), torch.randn(rows, generator=g).to(dev), torch.randn(rows, 3, generator=g).to(dev)]
+
+    def grad(up):
+        leaf = x.to(dev).requires_grad_(True)
+        got = label_log_probs(leaf, y.to(dev), top_k=3)
+        return torch.autograd.grad([got.log_prob, got.entropy, got.top_log_probs], leaf, up)[0]
+
+    want = grad([-u for u in ups])
+    lazy = [torch._neg_view(u) for u in ups]
+    assert all(u.is_neg() and u.is_contiguous() for u in lazy)
+    assert torch.equal(grad(lazy), want)
+    strided = [torch.complex(torch.zeros_like(u), u).conj().imag for u in ups]
+    assert all(u.is_neg() for u in strided)
+    assert torch.equal(grad(strided), want)
+    # and as autograd makes them by itself
+    leaf, plain = (x.to(dev).requires_grad_(True) for _ in range(2))
+    lp = label_log_probs(leaf, y.to(dev)).log_prob
+    torch.complex(torch.zeros_like(lp), lp).conj().imag.sum().backward()
+    (-label_log_probs(plain, y.to(dev)).log_prob).sum().backward()
+    assert torch.equal(leaf.grad, plain.grad)
 
 
 # ------------------------------------------------------------------------------------------------- embedding gradient
