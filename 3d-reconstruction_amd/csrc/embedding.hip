@@ -14,6 +14,7 @@
 // Up to EMB_DIRECT ids need no sort (but on a very large table): each workgroup picks the ids that fall among its rows.
 // Nor does a table of few and short rows, however many ids: it is added up in LDS.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "dtype_io.hpp"
@@ -772,8 +773,19 @@ __global__ __launch_bounds__(1024) void embed_few_join_kernel(int words, int blo
   __syncthreads();
   if (slice == 0 && e < words) {
     for (int k = 1; k < 32; ++k) acc += lds[k][threadIdx.x];
-    v_table[e] = (T)(acc * scale);
+    v_table[e] = (T)(acc * scale + 0.f);  // (+0 for a sum of nothing, whatever the sign of the scale)
   }
+}
+
+// A row that no id selects is zeros; its sum alone does not tell it from a selected row whose values add up to zero, which
+// differs only where 0 * scale is no zero.  With such a scale (infinite or NaN) this follows: a workgroup for each row looks
+// for an id of its own.
+template <typename T>
+__global__ __launch_bounds__(EMB_THREADS) void embed_few_unselected_kernel(EmbFew sh, const void* __restrict__ ids, int id_bytes,
+                                                                           T* __restrict__ v_table) {
+  bool any = false;
+  for (int64_t i = threadIdx.x; i < sh.n && !any; i += EMB_THREADS) any = emb_id(ids, id_bytes, i) == (int64_t)blockIdx.x;
+  if (!__syncthreads_or(any ? 1 : 0) && (int)threadIdx.x < sh.D) v_table[(int64_t)blockIdx.x * sh.D + threadIdx.x] = (T)0.f;
 }
 
 // Few ids: one launch.  The workgroup lists, in order, the ids that fall among its rows; each group adds those of its row.
@@ -840,7 +852,7 @@ __global__ __launch_bounds__(EMB_THREADS) void embed_direct_kernel(EmbShape sh, 
 #pragma unroll
           for (int k = 0; k < N; ++k) acc[k] += x[u][k];
     }
-    emb_store<T, N, false>(v_table + (v0 + r) * sh.vpr * N + vec * N, acc, sh.scale);
+    emb_store<T, N, false>(v_table + (v0 + r) * sh.vpr * N + vec * N, acc, s < e ? sh.scale : 0.f);  // (0 * scale may be NaN)
   }
 }
 
@@ -1055,6 +1067,11 @@ extern "C" int gs_embedding_bwd(int64_t n, int64_t V, int64_t D, int32_t dtype, 
             hipLaunchKernelGGL(embed_few_join_kernel<T>, dim3((unsigned)ceil_div(words, 32)), dim3(1024), 0, s, words,
                                (int)blocks, scale, (const float*)workspace, (T*)v_table);
             GS_CHECK_LAUNCH();
+            if (!std::isfinite(scale)) {
+              hipLaunchKernelGGL(embed_few_unselected_kernel<T>, dim3((unsigned)V), dim3(EMB_THREADS), 0, s, few, ids, id_bytes,
+                                 (T*)v_table);
+              GS_CHECK_LAUNCH();
+            }
             return GS_OK;
           }
           return GS_ERR_INVALID_ARG;

@@ -49,3 +49,27 @@ def test_a_table_without_rows(gpu_device, n, D):
     assert out.shape == (n, D) and bool((out == 0).all())
     out.sum().backward()
     assert table.grad.shape == (0, D)
+
+
+@pytest.mark.parametrize("scale", [float("inf"), float("-inf"), float("nan"), -2.0])
+@pytest.mark.parametrize("n,V,D", [(100, 50, 8), (256, 600, 3), (5000, 40, 16), (300_000, 64, 16), (5000, 90, 16), (300_000, 90, 16)])
+def test_rows_that_no_id_selects_are_zeros_whatever_the_scale(gpu_device, n, V, D, scale):
+    from gsplat.prepass import embedding_lookup
+
+    dev = gpu_device
+    g = torch.Generator().manual_seed(n + V)
+    ids = torch.randint(0, V, (n,), generator=g)
+    ids[(ids % 3) == 1] = -1  # a third of the rows is selected by nothing
+    up = torch.randn(n, D, generator=g)
+    up[ids == 0] = 0.0  # a selected row whose sum is zero
+    table = torch.zeros(V, D, device=dev, requires_grad=True)
+    (v,) = torch.autograd.grad(embedding_lookup(table, ids.to(dev), scale), table, up.to(dev))
+    v = v.cpu()
+    none = torch.bincount(ids[ids >= 0], minlength=V) == 0
+    assert bool(none.any()) and not bool(none.all())
+    assert bool((v[none] == 0).all()) and not bool(torch.signbit(v[none]).any())
+    if scale == -2.0:
+        assert bool((v[0] == 0).all()) and bool((v[~none][1:] != 0).any())
+    else:
+        assert bool(torch.isnan(v[0]).all()) if not bool(none[0]) else True
+        assert not bool(torch.isfinite(v[~none]).any())
