@@ -170,6 +170,7 @@ struct EmbeddingLookup : torch::autograd::Function<EmbeddingLookup> {
 Tensor embedding_lookup(const Tensor& table, const Tensor& ids, double scale) {
   dtype_code(table);
   index_bytes(ids);
+  TORCH_CHECK_VALUE(table.dim() == 2, "table must be [V,D], got ", table.sizes());
   require_gpu(table, table);
   require_gpu(ids, table);
   return EmbeddingLookup::apply(table, ids, scale);
@@ -220,6 +221,9 @@ struct LabelLogProbs : torch::autograd::Function<LabelLogProbs> {
 variable_list label_log_probs(const Tensor& logits, const Tensor& labels, int64_t top_k) {
   dtype_code(logits);
   index_bytes(labels);
+  // (the kernels read a label for each row: not left to Python's assertions, which can be switched off)
+  TORCH_CHECK_VALUE(logits.dim() >= 1 && labels.sizes() == logits.sizes().slice(0, logits.dim() - 1), "labels must be ",
+                    logits.sizes(), " without the last dimension, got ", labels.sizes());
   require_gpu(logits, logits);
   require_gpu(labels, logits);
   const bool flat = logits.dim() == 2;
