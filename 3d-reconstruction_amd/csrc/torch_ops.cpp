@@ -12,6 +12,7 @@
 #include <torch/csrc/autograd/graph_task.h>
 #include <torch/extension.h>
 
+#include <atomic>
 #include <unordered_set>
 
 #include "../../include/gsplat_mi355x.h"
@@ -88,6 +89,43 @@ struct Launch {
   explicit Launch(const Tensor& t) : guard(t.device()), stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
 };
 
+// The package's timing brackets (gsplat._backend.timed) around the launch of a backward, which has no Python around it.
+std::atomic<bool> timing{false};
+PyObject* timed = nullptr;  // the class while timing is on; read and written with the interpreter's lock
+
+void set_timed(const pybind11::object& cls) {
+  PyObject* const before = timed;
+  timed = cls.is_none() ? nullptr : cls.inc_ref().ptr();
+  timing = timed != nullptr;
+  Py_XDECREF(before);
+}
+
+class Bracket {
+  PyObject* guard = nullptr;
+
+ public:
+  Bracket(const char* name, const Tensor& t) {
+    if (!timing.load(std::memory_order_relaxed)) return;
+    const pybind11::gil_scoped_acquire lock;
+    if (!timed) return;
+    auto g = pybind11::reinterpret_borrow<pybind11::object>(timed)(name, t.device());
+    g.attr("__enter__")();
+    guard = g.release().ptr();
+  }
+  Bracket(const Bracket&) = delete;
+  Bracket& operator=(const Bracket&) = delete;
+  ~Bracket() {
+    if (!guard) return;
+    const pybind11::gil_scoped_acquire lock;
+    const auto g = pybind11::reinterpret_steal<pybind11::object>(guard);
+    try {
+      g.attr("__exit__")(pybind11::none(), pybind11::none(), pybind11::none());
+    } catch (pybind11::error_already_set& e) {
+      e.discard_as_unraisable("gsplat timing");
+    }
+  }
+};
+
 Tensor bytes(int64_t n, const Tensor& like) { return at::empty({n}, like.options().dtype(at::kByte)); }
 
 // dense rows with their elements next to each other, in memory as they are (a lazily negated view is not)
@@ -160,6 +198,7 @@ struct EmbeddingLookup : torch::autograd::Function<EmbeddingLookup> {
     const int64_t nbytes = L.embedding_bwd_workspace_bytes(n, V, D);
     const Tensor ws = nbytes ? bytes(nbytes, v) : Tensor();
     Launch on(v);
+    const Bracket bracket("gs_embedding_bwd", v);
     check(L.embedding_bwd(n, V, D, dtype_code(v), flat.data_ptr(), index_bytes(flat), v.data_ptr(), v.stride(0), (float)scale,
                           nbytes ? ws.data_ptr() : nullptr, nbytes, v_table.data_ptr(), on.stream), "gs_embedding_bwd");
     if (at::GradMode::is_enabled() && grads[0].requires_grad()) v_table = once(v_table, "embedding_lookup");
@@ -210,6 +249,7 @@ struct LabelLogProbs : torch::autograd::Function<LabelLogProbs> {
     Tensor v = at::empty({rows, K}, x.options());
     auto ptr = [](const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; };
     Launch on(x);
+    const Bracket bracket("gs_label_log_probs_bwd", x);
     check(L.label_bwd(rows, (int32_t)K, dtype_code(x), (int32_t)top_k, x.data_ptr(), x.stride(0), y.data_ptr(),
                       index_bytes(y), stats.data_ptr<float>(), entropy.data_ptr<float>(), top_idx.data_ptr<int64_t>(),
                       ptr(g[0]), ptr(g[1]), ptr(g[2]), v.data_ptr(), on.stream), "gs_label_log_probs_bwd");
@@ -340,6 +380,7 @@ std::pair<std::vector<Tensor>, Tensor> clip(const std::vector<Tensor>& grads, do
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   const auto free = pybind11::call_guard<pybind11::gil_scoped_release>();
   m.def("load", &load);
+  m.def("set_timed", &set_timed);
   m.def("embedding_lookup", &embedding_lookup, free);
   m.def("label_log_probs", &label_log_probs, free);
   m.def("grad_norm", &grad_norm, free);

@@ -258,6 +258,8 @@ def profiling_start(only=None) -> None:
     global _prof, _prof_only
     _prof = {}
     _prof_only = set(only) if only is not None else None
+    if _ops is not None:
+        _ops.set_timed(timed)
 
 
 def profiling_active(label: Optional[str] = None) -> bool:
@@ -272,6 +274,8 @@ def profiling_stop():
     """Returns {entry point: (calls, mean ms)}; synchronises the device once."""
     global _prof
     rec, _prof = _prof, None
+    if _ops is not None:
+        _ops.set_timed(None)
     if not rec:
         return {}
     torch.cuda.synchronize()
@@ -319,6 +323,8 @@ def ops():
         module = module_from_spec(spec)
         spec.loader.exec_module(module)
         module.load(lib_path())
+        if _prof is not None:
+            module.set_timed(timed)
         _ops = module
     return _ops
 

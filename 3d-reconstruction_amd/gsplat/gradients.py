@@ -26,7 +26,9 @@ def _listed(grads) -> List[Tensor]:
 
 def grad_norm(grads: Iterable[Tensor]) -> Tensor:
     """sqrt of the sum of squares over all tensors (fp32, bf16 and fp16, any mix) as a 0-d fp32 tensor on their device."""
-    return B.ops().grad_norm(_listed(grads))
+    grads = _listed(grads)
+    with B.timed("gs_grad_norm", grads[0].device if grads else None):
+        return B.ops().grad_norm(grads)
 
 
 def clip_gradients(grads: Iterable[Tensor], max_norm: float, inplace: bool = False,

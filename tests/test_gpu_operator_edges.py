@@ -73,3 +73,37 @@ def test_rows_that_no_id_selects_are_zeros_whatever_the_scale(gpu_device, n, V, 
     else:
         assert bool(torch.isnan(v[0]).all()) if not bool(none[0]) else True
         assert not bool(torch.isfinite(v[~none]).any())
+
+
+# ------------------------------------------------------------------------------------------------- timing
+def test_every_entry_point_is_timed(gpu_device):
+    from gsplat import _backend as B
+    from gsplat.gradients import clip_gradients, grad_norm
+    from gsplat.losses import label_log_probs
+    from gsplat.prepass import embedding_lookup
+
+    dev = gpu_device
+    table = torch.randn(50, 12, device=dev, requires_grad=True)
+    ids = torch.arange(5000, device=dev) % 50
+
+    def step():
+        out = embedding_lookup(table, ids)
+        (v,) = torch.autograd.grad(label_log_probs(out, ids % 12, 2).log_prob.sum(), table)
+        clip_gradients([v], 1.0)
+        return grad_norm([v])
+
+    want = step()
+    names = {"gs_embedding_fwd", "gs_embedding_bwd", "gs_label_log_probs_fwd", "gs_label_log_probs_bwd", "gs_grad_clip", "gs_grad_norm"}
+    B.profiling_start()
+    try:
+        step()
+        assert torch.equal(step(), want)
+    finally:
+        seen = B.profiling_stop()
+    assert set(seen) == names
+    assert all(calls == 2 and 0.0 <= ms < 1e3 for calls, ms in seen.values()), seen
+    B.profiling_start(only=["gs_label_log_probs_bwd"])
+    step()
+    assert set(B.profiling_stop()) == {"gs_label_log_probs_bwd"}
+    step()
+    assert B.profiling_stop() == {}
