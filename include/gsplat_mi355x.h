@@ -715,11 +715,13 @@ int gs_label_log_probs_fwd(int64_t rows, int32_t K, int32_t dtype, int32_t top_k
                            float* log_prob /* [rows] */, float* entropy /* [rows] */, float* stats /* [rows,2] */,
                            float* top_log_probs /* [rows,top_k] */, int64_t* top_labels /* [rows,top_k] */, void* stream);
 /* v_logits [rows,K] (dense, written whole) from the gradients of log_prob, entropy and top_log_probs, each of which may
- * be NULL.  Labels outside [0, K) and rows of nothing but -inf pass nothing on. */
+ * be NULL; `stats`, `entropy` and `top_labels` as the forward wrote them for the same logits (top_labels may be NULL where
+ * g_top_log_probs is).  Labels outside [0, K) and rows of nothing but -inf pass nothing on. */
 int gs_label_log_probs_bwd(int64_t rows, int32_t K, int32_t dtype, int32_t top_k, const void* logits, int64_t row_stride,
-                           const void* labels, int32_t label_bytes, const float* lse, const float* entropy,
-                           const int64_t* top_labels, const float* g_log_prob, const float* g_entropy,
-                           const float* g_top_log_probs, void* v_logits, void* stream);
+                           const void* labels, int32_t label_bytes, const float* stats /* [rows,2] */,
+                           const float* entropy /* [rows] */, const int64_t* top_labels /* [rows,top_k] */,
+                           const float* g_log_prob /* [rows] */, const float* g_entropy /* [rows] */,
+                           const float* g_top_log_probs /* [rows,top_k] */, void* v_logits, void* stream);
 
 /* ---- gradients of a step: global norm and clipping ------------------------------------------------------- */
 /* norm [1] = sqrt of the sum of squares over all tensors (64-bit sums, order fixed by the sizes).  The *_host arrays are

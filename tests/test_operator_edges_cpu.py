@@ -49,3 +49,24 @@ def test_shapes_are_checked_with_assertions_off_too(flags):
     package = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "3d-reconstruction_amd")
     run = subprocess.run([sys.executable, *flags, "-c", CALLS.format(package=package)], capture_output=True, text=True, timeout=300)
     assert [line.split()[:2] for line in run.stdout.splitlines()] == [[str(i), "refused:"] for i in range(6)], (run.stdout, run.stderr[-2000:])
+
+
+def test_the_header_names_what_the_kernels_read():
+    """Parameter names of the declarations are those of the definitions: a caller goes by the header alone."""
+    import os
+    import re
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+    def parameters(path, end):
+        with open(path) as f:
+            text = re.sub(r"/\*.*?\*/|//[^\n]*", "", f.read(), flags=re.S)
+        found = re.findall(r"\b(gs_(?:embedding|label|grad)_\w+)\s*\(([^()]*)\)\s*" + end, text)
+        return {name: [re.findall(r"\w+", p)[-1] for p in args.split(",")] for name, args in found}
+
+    declared = parameters(os.path.join(root, "include", "gsplat_mi355x.h"), ";")
+    defined = {}
+    for source in ("embedding.hip", "labels.hip", "gradients.hip"):
+        defined.update(parameters(os.path.join(root, "3d-reconstruction_amd", "csrc", source), "{"))
+    assert len(declared) == 9
+    assert declared == {name: defined[name] for name in declared}
