@@ -70,3 +70,17 @@ def test_the_header_names_what_the_kernels_read():
         defined.update(parameters(os.path.join(root, "3d-reconstruction_amd", "csrc", source), "{"))
     assert len(declared) == 9
     assert declared == {name: defined[name] for name in declared}
+
+
+def test_changed_build_flags_rebuild_everything():
+    """Flags that decide which instructions may be used stand in the Makefile: objects of older flags are not kept."""
+    import os
+    import subprocess
+
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "3d-reconstruction_amd", "csrc")
+    plan = subprocess.run(["make", "-n", "-W", "Makefile", "-C", csrc, "TORCH_FLAGS="], capture_output=True, text=True, timeout=120).stdout
+    sources = [f for f in os.listdir(csrc) if f.endswith(".hip")]
+    assert len(sources) >= 16
+    for f in sources:
+        assert f"-c {f} " in plan, f
+    assert "torch_ops.cpp" in plan
