@@ -1,10 +1,13 @@
-"""Calls of the embedding, label and gradient operators at the edges of what their documentation allows."""
+"""Calls of the embedding, label and gradient operators at the edges of what their documentation allows, and sums whose
+every partial sum is exact, so that a row left out anywhere shows."""
 import pytest
 import torch
 
-from test_gpu_labels import _case
+from test_gpu_labels import _case, _check
 
 pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
 
 
 # ------------------------------------------------------------------------------------------------- label gradient
@@ -73,6 +76,120 @@ def test_rows_that_no_id_selects_are_zeros_whatever_the_scale(gpu_device, n, V, 
     else:
         assert bool(torch.isnan(v[0]).all()) if not bool(none[0]) else True
         assert not bool(torch.isfinite(v[~none]).any())
+
+
+def _exact_sums(ids, values, V):
+    """Sums of integer rows in 64 bits, over the ids in [0, V): differences of the running sums of the sorted rows."""
+    keep = (ids >= 0) & (ids < V)
+    s, order = ids[keep].sort()
+    run = torch.nn.functional.pad(values[keep][order].double().t().contiguous().cumsum(1), (1, 0))
+    cut = torch.searchsorted(s, torch.arange(V + 1, device=ids.device))
+    return (run[:, cut[1:]] - run[:, cut[:-1]]).t()
+
+
+def _whole_rows(n, D, dtype, dev):
+    """Values of -2 to 2: with a power of two as the scale every sum of up to 2^22 of them is exact in fp32, in any order."""
+    assert n <= 1 << 22
+    up = torch.randint(-2, 3, (n, D), generator=torch.Generator(device=dev).manual_seed(n), device=dev).to(dtype)
+    up[:, 0] = 1.0  # a count: no two rows can stand in for each other
+    return up
+
+
+def _check_exact(name, ids, V, up):
+    from gsplat.prepass import embedding_lookup
+
+    table = torch.zeros(V, up.shape[1], device=up.device, dtype=up.dtype, requires_grad=True)
+    (v,) = torch.autograd.grad(embedding_lookup(table, ids, 0.5), table, up)
+    want = (_exact_sums(ids, up, V) * 0.5).float().to(up.dtype)
+    assert torch.equal(v, want), f"{name}: {int((v != want).sum())} of {v.numel()} differ"
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,V,D", [(257, 64, 1), (5000, 1, 128), (300_000, 64, 16), (300_000, 3, 5), (1_000_000, 8, 100),
+                                   (16_384, 70, 20), (16_385, 70, 20), (40_000, 5000, 24), (70_001, 300, 33), (300_000, 65, 16),
+                                   (131_072, 70_000, 8), (100_003, 1000, 704), (20_000, 7, 300), (5000, 1, 256), (66_000, 1 << 20, 2),
+                                   (1_000_000, 200_000, 16), (1_000_001, 65, 7)])
+@pytest.mark.parametrize("kind", ["uniform", "grouped", "few", "one", "outside"])
+def test_no_row_is_left_out_of_a_sum(gpu_device, n, V, D, dtype, kind):
+    g = torch.Generator().manual_seed(n + V)
+    if kind == "one":
+        ids = torch.full((n,), V - 1, dtype=torch.int64)
+    elif kind == "few":
+        ids = torch.randint(0, 3, (n,), generator=g) * (V // 3)
+    else:
+        ids = torch.randint(0, V, (n,), generator=g)
+    if kind == "grouped":
+        ids = ids.sort().values
+    elif kind == "outside":
+        ids[torch.rand(n, generator=g) < 0.5] = -1
+    _check_exact(f"{dtype} {n}x{V}x{D} {kind}", ids.to(gpu_device), V, _whole_rows(n, D, dtype, gpu_device))
+
+
+@pytest.mark.parametrize("n,V,D", [(4000, 100, 16), (40_000, 100, 16), (140_000, 70, 3), (140_000, 300, 64), (20_000, 500, 260),
+                                   (60_000, 90, 1200), (1_200_000, 100, 16)])
+def test_no_row_is_left_out_of_a_long_run(gpu_device, n, V, D):
+    """Runs that start and end anywhere in what one workgroup has, up to all ids but a few."""
+    dev = gpu_device
+    g, up = torch.Generator(device=dev).manual_seed(n + D), _whole_rows(n, D, torch.float32, dev)
+    for lead in (0, 1, 15, 64, 257, 1024, 4097):
+        for length in (16, 17, 63, 64, 65, 256, 257, 511, 1024, 1500, 4096, 8191, n // 2, n - 3000, n - lead - 1, n - lead):
+            if length < 1 or lead + length > n:
+                continue
+            ids = torch.full((n,), V - 1, device=dev)
+            ids[:lead] = torch.arange(lead, device=dev) % (V // 3)
+            ids[lead:lead + length] = V // 2
+            rest = n - lead - length
+            ids[lead + length:] = V // 2 + 1 + torch.arange(rest, device=dev) % (V - V // 2 - 1)
+            ids = ids[torch.randperm(n, generator=g, device=dev)]
+            _check_exact(f"run of {length} behind {lead} of {n}x{V}x{D}", ids, V, up)
+
+
+def test_values_behind_32_bits(gpu_device):
+    """The gradient of a table of more than 2^31 elements: every row that was selected, and nothing else."""
+    from gsplat.prepass import embedding_lookup
+
+    dev, V, D = gpu_device, 1_100_000, 2048
+    table = torch.zeros(V, D, device=dev, dtype=torch.bfloat16, requires_grad=True)
+    rows = torch.tensor([V - 1, 0, V - 2], device=dev)
+    out = embedding_lookup(table, rows.repeat(200))
+    (v,) = torch.autograd.grad(out, table, torch.ones_like(out))
+    assert bool((v[rows] == 200).all())
+    assert sorted((v != 0).any(1).nonzero()[:, 0].tolist()) == sorted(rows.tolist())
+
+
+# ------------------------------------------------------------------------------------------------- alternatives
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("K", [66, 100, 129, 160, 200, 255, 299, 511])
+@pytest.mark.parametrize("top", [9, 17, 21, 32, 33, 64])
+def test_many_alternatives_of_middling_rows(gpu_device, K, top, dtype):
+    """More of them than lanes that hold values, in rows of ordinary values."""
+    x, y, _ = _case(37, K, dtype, K + top)
+    _check(f"{dtype} 37x{K} top {top}", gpu_device, x, y, top=top)
+
+
+# ------------------------------------------------------------------------------------------------- clipping
+@pytest.mark.parametrize("inplace", [False, True])
+def test_a_captured_clip_within_and_beyond_the_limit(gpu_device, inplace):
+    from gsplat.gradients import clip_gradients
+
+    dev = gpu_device
+    raw = [torch.randn(n, device=dev).to(t) for n, t in ((50_001, torch.float32), (3, torch.bfloat16), (4099, torch.float16))]
+    work = [t.clone() for t in raw]
+    clip_gradients([t.clone() for t in raw], 1.0, inplace=inplace)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured, norm = clip_gradients(work, 1.0, inplace=inplace)
+    for k, scale in enumerate((1e-4, 1.0, 1e-3, 30.0, 1e-4)):
+        for t, w in zip(raw, work):
+            t.normal_().mul_(scale)
+            w.copy_(t)
+        want, n = clip_gradients(raw, 1.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert (float(n) < 1.0) == (scale < 1e-2), (k, float(n))
+        assert torch.equal(norm, n) and all(torch.equal(a, b) for a, b in zip(captured, want)), k
+        if scale < 1e-2:
+            assert all(torch.equal(a, b) for a, b in zip(captured, raw)), k
 
 
 # ------------------------------------------------------------------------------------------------- timing
