@@ -3,7 +3,8 @@ every partial sum is exact, so that a row left out anywhere shows."""
 import pytest
 import torch
 
-from test_gpu_labels import _case, _check
+from operator_bounds import assert_within, rounding
+from test_gpu_labels import _case, _check, _reference
 
 pytestmark = pytest.mark.gpu
 
@@ -165,6 +166,86 @@ def test_many_alternatives_of_middling_rows(gpu_device, K, top, dtype):
     """More of them than lanes that hold values, in rows of ordinary values."""
     x, y, _ = _case(37, K, dtype, K + top)
     _check(f"{dtype} 37x{K} top {top}", gpu_device, x, y, top=top)
+
+
+@pytest.mark.parametrize("rows,K,dtype,top", [(2_000_003, 19, torch.float32, 3), (2_000_003, 63, torch.bfloat16, 2),
+                                              (40_001, 1001, torch.float32, 5), (80_000, 1999, torch.bfloat16, 33),
+                                              (300, 120_001, torch.float32, 64), (2000, 40_001, torch.float16, 8)])
+def test_large_gradients_with_alternatives(gpu_device, rows, K, dtype, top):
+    """Gradients that are stored past the caches, with the alternatives' terms stored behind them."""
+    from gsplat.losses import label_log_probs
+
+    dev = gpu_device
+    g = torch.Generator(device=dev).manual_seed(rows)
+    x = (torch.randn(rows, K, device=dev, generator=g) * 3).to(dtype).requires_grad_(True)
+    y = torch.randint(-1, K, (rows,), device=dev, generator=g)
+    ups = [torch.randn(rows, device=dev, generator=g), torch.randn(rows, device=dev, generator=g), torch.randn(rows, top, device=dev, generator=g)]
+    got = label_log_probs(x, y, top)
+    (v,) = torch.autograd.grad([got.log_prob, got.entropy, got.top_log_probs], x, ups)
+    some = torch.cat([torch.arange(4), torch.randint(0, rows, (8,)), torch.arange(rows - 4, rows)]).to(dev)
+    ref = _reference(x.detach()[some], y[some], top, *(u[some] for u in ups))
+    assert torch.equal(got.top_labels[some].cpu(), ref["top_labels"])
+    assert_within(f"{rows}x{K} {dtype} v", v[some], ref["v"][0], ref["v"][1] + rounding(dtype, ref["v"][0]))
+
+
+def test_saved_tensors_that_travel_and_graphs_that_stay(gpu_device):
+    """What the backward needs may be kept elsewhere meanwhile; a graph can be walked twice; no graph is made where none is."""
+    from gsplat.losses import label_log_probs
+    from gsplat.prepass import embedding_lookup
+
+    dev = gpu_device
+    table = torch.randn(700, 40, device=dev, requires_grad=True)
+    ids = torch.randint(-1, 700, (9000,), device=dev)
+    render = torch.randn(9000, 60, device=dev, requires_grad=True)
+
+    def step():
+        got = label_log_probs(embedding_lookup(table, ids) + render[:, 7:47], ids % 40, 4)
+        return got.log_prob.sum() + got.entropy.sum() + got.top_log_probs.sum(), got
+
+    def sliced():
+        got = label_log_probs(render[:, 3:43], ids % 40, 4)
+        return got.log_prob.sum() + got.top_log_probs.sum(), got
+
+    for make, leaves in ((step, [table, render]), (sliced, [render])):
+        loss, got = make()
+        want = torch.autograd.grad(loss, leaves, retain_graph=True)
+        again = torch.autograd.grad(loss, leaves)
+        assert all(torch.equal(a, b) for a, b in zip(want, again))
+        with torch.autograd.graph.save_on_cpu():
+            loss, _ = make()
+        assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(loss, leaves)))
+        with torch.inference_mode():
+            _, plain = make()
+        assert all(torch.equal(a, b) and not b.requires_grad for a, b in zip(got, plain))
+
+
+def test_long_sort_and_alternatives_in_a_graph(gpu_device):
+    from gsplat.losses import label_log_probs
+    from gsplat.prepass import embedding_lookup
+
+    dev, n, V, D = gpu_device, 40_000, 3000, 130
+    table = torch.randn(V, D, device=dev, requires_grad=True)
+    ids, up = torch.randint(0, V, (n,), device=dev), torch.randn(n, 40, device=dev)
+
+    def step():
+        got = label_log_probs(embedding_lookup(table, ids, 0.5), ids % D, 40)
+        return [got.log_prob, got.top_labels, torch.autograd.grad([got.log_prob, got.top_log_probs], table, [up[:, 0], up])[0]]
+
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream(dev).wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for k in range(4):
+        with torch.no_grad():
+            table.normal_(), up.normal_(), ids.random_(-1, V + 1)
+        want = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, want)), k
 
 
 # ------------------------------------------------------------------------------------------------- clipping
