@@ -1,6 +1,6 @@
 // Embedding lookup with scaling, and the gradient of the table by sorted ids.
 //   out[i] = scale * table[ids[i]]                          (an id outside [0, V) selects nothing: a row of zeros)
-//   v_table[v] = scale * sum over i with ids[i] = v, in ascending i, of v_out[i]
+//   v_table[v] = scale * sum over i with ids[i] = v of v_out[i]   (a row that no id selects: zeros, whatever the scale)
 // Both are bound by HBM.  The lookup reads n rows and writes n rows in the widest vectors that the row size and the
 // alignment allow.  The gradient reads every row of v_out once and writes the table:
 //   1. the ids are sorted, stably, with their positions: by one workgroup in LDS up to EMB_SORT1 of them, else by a radix
@@ -10,7 +10,9 @@
 //      ids is added up by the group in whose piece it starts, and stored; of a long one each group adds what lies in its
 //      piece.
 //   3. embed_join_kernel adds the pieces of each long run.
-// Sums are held in fp32, taken in an order that the ids alone fix (no float atomics), and rounded once at the end.
+// Sums are held in fp32 and rounded once at the end.  Their order is fixed (no float atomics) by the ids, the sizes and the
+// width of the vectors that strides and addresses allow: ascending i in a short run, groups and workgroups joined as trees in a
+// long one, threads' shares in a table of few rows.
 // Up to EMB_DIRECT ids need no sort (but on a very large table): each workgroup picks the ids that fall among its rows.
 // Nor does a table of few and short rows, however many ids: it is added up in LDS.
 #include <algorithm>
@@ -140,6 +142,9 @@ __device__ __forceinline__ void emb_fill(const EmbFill& f, int64_t block, int64_
 }
 
 // ---- stable sort of the ids with their positions
+// Not radix_sort.hip's: that one sorts 64-bit keys (tile and depth) from given pairs, with the count in device memory, and has
+// no room for the table's zeros.  Here keys are one word and the first digit's come straight from the ids, and a tile scatters
+// through LDS, which pays for the few digits that ids have: 1M items, a digit of 9 bits 14 us against 24 from registers.
 __device__ __forceinline__ uint32_t emb_key(const void* ids, int id_bytes, int64_t i, int64_t V) {
   const int64_t id = emb_id(ids, id_bytes, i);
   return id >= 0 && id < V ? (uint32_t)id : (uint32_t)V;  // ids that select nothing sort behind all rows
@@ -701,7 +706,9 @@ __global__ __launch_bounds__(EMB_JOIN_THREADS) void embed_join_kernel(EmbShape s
 // each, and add them to a table in LDS that belongs to the thread's place among those rows: no two threads meet in a word.
 // Equal ids in succession, the rule where Gaussians lie instance by instance, add up in a register first.  The tables of a
 // workgroup are added up, in their order, and embed_few_join_kernel adds the workgroups'.
-// 1M x 16 fp32 on 64 rows: 24 + 4 us (3.0 TB/s; LDS leaves a CU eight waves), against 55 us by the sort.
+// 1M x 16 fp32 on 64 rows: 23 + 4 us (3.0 TB/s; these tables, 64 KiB a workgroup, leave a CU eight waves), against 55 us by
+// the sort; on 8 rows 20 + 4 us.  A thread adds up to n Dp / 131072 values of a row one after another: fp32 as all sums here, but
+// with an error that grows with n.
 struct EmbFew {
   int64_t n, per, gs;   // ids, ids of a workgroup, row stride of v_out
   int32_t V, D, Dp;     // Dp: D rounded up to a power of two

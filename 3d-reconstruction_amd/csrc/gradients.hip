@@ -4,7 +4,8 @@
 // The table of tensors (pointers, sizes, types) travels in the kernel arguments: nothing is copied to the device, so a
 // call can be captured, and nothing outlives it.  A launch carries 128 tensors; more take further launches.
 // The squares are summed in 64 bits (a square leaves the range of fp32 from 1.8e19 up and from 1e-19 down) in an order
-// that the sizes alone fix: equal gradients give equal bits on every rank.  The 64-bit sums cost nothing that shows: 708 MB of
+// that the sizes, the order in memory and the distance from a 16-byte boundary fix: ranks that lay equal gradients out alike get
+// equal bits.  The 64-bit sums cost nothing that shows: 708 MB of
 // fp32 are read in 113 us (6.3 TB/s), 537 MB of bf16 in 83 us (6.4).  The second pass takes 183 us for those 537 MB, read and
 // written (5.9 TB/s), and 5 us when nothing has to change.
 #include <algorithm>

@@ -29,6 +29,8 @@ constexpr int LP_LIST = 1024;      // candidates for the top alternatives that a
 constexpr float LP_LOG2E = 1.44269504088896340736f;
 constexpr float LP_LOW = -1.0e4f;  // stands for -inf next to an exponential that is 0 there: 0 * LP_LOW is 0
 
+// The hardware's 2^x of the rounded d log2 e: off by (2 |d| + 2) 2^-24 of itself at most, which grows with the distance from
+// the maximum as the term's weight falls (465750 x 19, all results against 64 bits: 8.5e-8, elementary torch operations 6.0e-8).
 __device__ __forceinline__ float lp_exp(float d) { return __builtin_amdgcn_exp2f(d * LP_LOG2E); }
 
 // max, sum of exp(x - max) and sum of exp(x - max) (x - max) of a part of a row.  m ignores NaN, which s and w keep; with
@@ -159,7 +161,9 @@ __device__ __forceinline__ void lp_write_top(const LpFwd& a, int64_t r, int rank
 // apart: lanes that each walk their own row hit different banks), and each lane works on one row without any exchange.
 // f / K for f < 64 K by a multiplication: (2^22 / K + 1) f is off by less than f / 2^22 < 1 / K.
 // 465750 x 19 fp32: 13 us (3.5 TB/s with labels and results) and 19 us for the gradient (3.7 TB/s of logits); bound by the
-// exponentials and LDS words of one lane a row.  Five best of a row cost K comparisons each.
+// exponentials and LDS words of one lane a row, so that 16-bit rows, staged and written value by value, take the same (13 and
+// 18 us for half the bytes).  Each alternative of a row costs K comparisons: 465750 x 19 with the five best 26 us, 300000 x 60
+// 28 us, with the ten best 102 us, with the twenty best 211 us; gradients 24, 44, 51 and 74 us.
 template <typename T>
 __device__ __forceinline__ void lp_small_load(const T* __restrict__ logits, int64_t stride, int64_t row0, int rows, int K,
                                               int P, uint32_t magic, int lane, float* __restrict__ tile) {
@@ -233,8 +237,12 @@ __global__ __launch_bounds__(64) void label_small_fwd_kernel(LpFwd a, uint32_t m
 // -------------------------------------------------------------------------------------------- up to LP_WAVE classes
 // A wave holds a row in registers: NV vectors a lane and one extra value.  Read once, whatever is asked for.
 // 8191 x 1000 fp32 with the five best 11 us (3.0 TB/s), a quarter of it for the alternatives, and 19 us where just three
-// classes are not ruled out; bound by instructions, six waves on a SIMD (forced to eight, with values spilled, 16 us).  Four
-// at least: 8191 x 2048 bf16 with the twenty best 20 us, three waves 25.
+// classes are not ruled out; bound by the instructions that every row takes whatever its length (reductions, the search for
+// the threshold, listing), so that short rows are far from the bytes: 300000 x 100 76 us (1.6 TB/s), 16-bit 95 us, 200000 x 500
+// 87 us (4.6 TB/s).  With more alternatives than lanes that hold values the whole row is listed: 300000 x 100 bf16 with the
+// twenty best 641 us, and 300000 x 160 with 21, where the list overflows and they are taken one by one, 1483 us (fp32, whose
+// rows fill twice the lanes, 208 us).  Six waves on a SIMD (forced to eight, with values spilled, 16 us); four at least: 8191 x
+// 2048 bf16 with the twenty best 20 us, three waves 25.
 // f(value, index) over thread t's strip: every LANES-th vector
 template <int LANES, typename T, typename F> __device__ __forceinline__ void lp_walk(const LpSpan<T>& sp, int t, F&& f) {
   constexpr int VE = LpSpan<T>::VE;
@@ -772,8 +780,10 @@ __global__ __launch_bounds__(64) void label_small_bwd_kernel(LpBwd a, uint32_t m
 }
 
 // LANES threads (a wave, or a workgroup) over a part of a row; the gradient's row is as far apart from a 16-byte boundary
-// as the logits' (`wide`), or is written value by value.  2048 x 100277 bf16 in 8192 segments 163 us, 5.0 TB/s (one vector
-// in flight and a workgroup a row: 203 us).
+// as the logits' (`wide`), or is written value by value (a slice of channels, whose rows are not K apart).  2048 x 100277 bf16
+// in 8192 segments 163 us, 5.0 TB/s (one vector in flight and a workgroup a row: 203 us).  A wave a row is bound by the latency
+// of a row at a time: 300000 x 100 fp32 89 us (2.7 TB/s), bf16 123 us (1.0), 200000 x 500 148 and 89 us (5.4 and 4.5); with
+// alternatives, whose places are stored a second time behind a wait, 300000 x 100 with five 173 us, with twenty 292 us.
 template <typename T, int LANES, bool PAST>
 __device__ __forceinline__ void lp_grad_span(const LpSpan<T>& sp, const LpRow& w, int j0, int t, T* __restrict__ out) {
   constexpr int VE = LpSpan<T>::VE;

@@ -6,7 +6,8 @@ all tensors instead of several per tensor.
     norm = clip_grad_norm(params, max_norm=1.0)
     optimizer.step()
 
-The norm is a 64-bit sum in an order that the sizes alone fix: ranks that hold equal gradients get equal bits.
+The norm is a 64-bit sum in an order that sizes, layouts and alignment fix: ranks that hold equal gradients in equal
+layouts get equal bits.
 """
 from __future__ import annotations
 
@@ -34,11 +35,12 @@ def grad_norm(grads: Iterable[Tensor]) -> Tensor:
 def clip_gradients(grads: Iterable[Tensor], max_norm: float, inplace: bool = False,
                    error_if_nonfinite: bool = False) -> Tuple[List[Tensor], Tensor]:
     """Scales the gradients by `min(1, max_norm / (norm + 1e-6))`, `norm` being the one over all of them.  Returns (the
-    scaled gradients, norm as a 0-d fp32 tensor): new tensors (small ones in one allocation together), or with `inplace`
-    the same ones, which are neither read a second time nor written when the norm is within `max_norm`.  A NaN norm makes
-    every gradient NaN and an infinite one makes the finite ones 0; `error_if_nonfinite` raises instead, before anything is
-    changed (one host synchronisation and one more read of the gradients).  No two gradients may share memory when they
-    are scaled in place."""
+    scaled gradients, norm as a 0-d fp32 tensor): new tensors, or with `inplace` the same ones, which are neither read a
+    second time nor written when the norm is within `max_norm` (views with gaps are, through a copy).  Small new tensors
+    are pieces of one allocation, as those of `torch.split` are: `resize_` to more elements would reach into the next.  A
+    NaN norm makes every gradient NaN, and so does an infinite one with an infinite `max_norm`; with a finite one it makes
+    the finite values 0.  `error_if_nonfinite` raises instead, before anything is changed (one host synchronisation and one
+    more read of the gradients).  No two gradients may share memory when they are scaled in place."""
     grads = _listed(grads)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:

@@ -247,7 +247,8 @@ def embedding_lookup(table: Tensor, ids: Tensor, scale: float = 1.0, validate: b
     table [V,D] fp32, bf16 or fp16; ids of any shape, int64 or int32; returns [*ids.shape, D] in the table's type.  An id
     outside [0, V) (a Gaussian without an instance) gives a row of zeros and passes no gradient on; `validate=True` raises
     for one instead (one host synchronisation).  Differentiable once w.r.t. the table: the gradient is dense, each row the
-    sum over its ids in fp32, in an order that the ids alone fix: the same bits in every run."""
+    sum over its ids in fp32 (zeros where there are none), in an order that ids, sizes and alignment fix: the same bits in
+    every run."""
     assert table.dim() == 2, f"table must be [V,D], got {tuple(table.shape)}"
     if validate and ids.numel() > 0 and not bool(((ids >= 0) & (ids < table.shape[0])).all()):
         raise IndexError(f"ids outside [0, {table.shape[0]})")

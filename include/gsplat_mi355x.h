@@ -695,7 +695,8 @@ int gs_cube_texture_bwd(int64_t n, int32_t R, int32_t C, const float* dirs, cons
 int gs_embedding_fwd(int64_t n, int64_t V, int64_t D, int32_t dtype, const void* table, int64_t table_stride,
                      const void* ids, int32_t id_bytes, float scale, void* out, void* stream);
 /* v_table [V,D] (dense, written whole) = scale * the sum of the v_out rows (v_out_stride elements apart) of each id.
- * Sums in fp32, in an order the ids alone fix, rounded once.  n < 2^30, V < 2^31, D up to 4M vectors of 16 bytes. */
+ * Rows of no id are zeros, whatever the scale.  Sums in fp32, in an order that the ids, the sizes and the alignment of
+ * v_out and its rows fix, rounded once.  n < 2^30, V < 2^31, D up to 4M vectors of 16 bytes. */
 int64_t gs_embedding_bwd_workspace_bytes(int64_t n, int64_t V, int64_t D);
 int gs_embedding_bwd(int64_t n, int64_t V, int64_t D, int32_t dtype, const void* ids, int32_t id_bytes,
                      const void* v_out, int64_t v_out_stride, float scale, void* workspace /* 16-B aligned */,
@@ -724,7 +725,7 @@ int gs_label_log_probs_bwd(int64_t rows, int32_t K, int32_t dtype, int32_t top_k
                            const float* g_top_log_probs /* [rows,top_k] */, void* v_logits, void* stream);
 
 /* ---- gradients of a step: global norm and clipping ------------------------------------------------------- */
-/* norm [1] = sqrt of the sum of squares over all tensors (64-bit sums, order fixed by the sizes).  The *_host arrays are
+/* norm [1] = sqrt of the sum of squares over all tensors (64-bit sums, order fixed by sizes and alignment).  The *_host arrays are
  * HOST arrays of n_tensors device pointers, element counts and GS_DTYPE_* codes; they are read before the call returns. */
 int64_t gs_grad_norm_workspace_bytes(int32_t n_tensors);
 int gs_grad_norm(int32_t n_tensors, const void* const* src_host, const int64_t* numel_host, const int32_t* dtype_host,
